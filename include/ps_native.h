@@ -128,7 +128,8 @@ int ps_store_set_updater(ps_store_t *s, const char *key_or_prefix, const ps_upda
 
 /* KVStore.get(key) / put(key,val) by reference-style string key:
  *   "emF<f>.<id>.0" (D floats), "wide.weights.<id>.0" (1), "wide.bias" (1),
- *   "fc<i>.weights" (out*in, reference layout [in][out]), "fc<i>.bias" (out).
+ *   "fc<i>.weights" (out*in, reference layout [in][out]), "fc<i>.bias" (out),
+ *   "ln<i>.weights", "ln<i>.bias" (dims; ps_store_create_ln).
  * get: *len receives the element count; PS_MISSING when the key is not
  * held by this shard (store/KVStore.java:129-134 returns null). */
 int ps_store_get(ps_store_t *s, const char *key, float *out, int cap, int *len);
@@ -171,7 +172,8 @@ enum { PS_GRAD_COMPAT = 0,     /* reference arithmetic incl. the double-backward
                                   factor (n+1)/(2n^2) and the
                                   "every wide key ever seen" gradient (A.10)   */
        PS_GRAD_INTENDED = 1    /* mean over occurrences / per-key presence sum */ };
-enum { PS_ACT_NONE = 0, PS_ACT_RELU = 1, PS_ACT_SIGMOID = 2 };
+enum { PS_ACT_NONE = 0, PS_ACT_RELU = 1, PS_ACT_SIGMOID = 2,
+       PS_ACT_GELU = 3, PS_ACT_SILU = 4   /* the residual tower's operators only (ps_fc_res_*): z Phi(z) and z / (1 + e^-z) */ };
 
 typedef struct ps_model_config {
     int kind;            /* PS_MODEL_*                                        */
@@ -314,8 +316,74 @@ int ps_fc_pending_grad(ps_store_t *s, int layer, int bias, float *out, int cap, 
  * (store/KVStore.java:240-277): g = pending sum / count, the updater resolved
  * for "fc<i>.weights" (exact key, prefix, "default"), W' and its transpose
  * rewritten, pending cleared, globalStep++.  layer < 0: every layer with a
- * pending gradient; a named layer without one: PS_MISSING. */
+ * pending gradient, normalisations (ps_ln_backward) among them; a named FC layer
+ * without one: PS_MISSING. */
 int ps_dense_update(ps_store_t *s, int layer);
+/* ---- the residual tower: layer normalisation, FC with bias, activation and
+ *      residual in one call ------------------------------------------------
+ * What a tower that grows deep or wide is stacked from, beside ps_fc_forward /
+ * ps_fc_backward (the reference has neither normalisation nor skip connections):
+ *   y = r + act(x W + b)        with x = LN(r) for the usual pre-norm block.
+ * Parameters are the store's, f32, under the store's keys: "fc<i>.*" as above
+ * and "ln<i>.weights" (gamma, ones at first) / "ln<i>.bias" (beta, zeros), which
+ * ps_store_get / put / key_length / push_update, set_updater, save and load know.
+ * ACTIVATIONS are of one type per call, PS_T_F32, PS_T_BF16 or PS_T_F16; a 16-bit
+ * product takes the weights, and the gradient dz behind the activation, rounded
+ * to that type.  Sums, statistics and parameter gradients are f32; every output
+ * is rounded once.
+ * x_dev etc. are [B][width] with a row stride ld >= width in ELEMENTS of the type,
+ * any stride and any alignment of the element's own size (16-byte aligned rows
+ * are fastest); nothing behind a row's width is read or written.  No ones column.
+ * Activations: PS_ACT_NONE, RELU, GELU, SILU (SIGMOID is the head's: PS_E_UNSUPPORTED).
+ * Outputs may not overlap inputs, except where a call says so: PS_E_BAD_ARG.
+ * Everything is enqueued on the store's stream; nothing waits for the device
+ * except a call that has to enlarge the store's workspace.
+ * HIP graphs: a call may be recorded (on a capturing stream adopted with
+ * ps_store_set_stream) once the same shapes have run eagerly -- the workspace
+ * does not grow while recording, PS_E_STATE -- and with grad_dev given: the
+ * pending gradient's count lives on the host, so a call that would add to it is
+ * refused while recording, PS_E_UNSUPPORTED.  The workspace is the store's: replays
+ * of its graphs are calls on the store, one at a time like all of them. */
+enum { PS_T_F32 = 0, PS_T_BF16 = 1, PS_T_F16 = 2 };
+/* "ln<layer>.weights" = 1 / "ln<layer>.bias" = 0, dims each; layer < 64, dims <= 2^20.
+ * Again with the same dims: nothing happens. */
+int ps_store_create_ln(ps_store_t *s, int layer, int dims);
+/* y = (x - mean) / sqrt(var + eps) * gamma + beta over each row (var: / dims), eps >= 0.
+ * stats_dev [B][2] (mean, 1 / sqrt(var + eps)) is what ps_ln_backward needs; NULL
+ * when serving.  y_dev may be x_dev (same ld). */
+int ps_ln_forward(ps_store_t *s, int layer, int type, const void *x_dev, int64_t ldx, int B, float eps,
+                  void *y_dev, int64_t ldy, float *stats_dev);
+/* x_dev / stats_dev as given to and left by ps_ln_forward, dy_dev the gradient wrt y:
+ *   dx_dev   (NULL: not wanted) = skip + d/dx, skip_dev [B][dims] or NULL: the
+ *            gradient that came round the normalisation on the residual path.
+ *            dx_dev may be dy_dev or skip_dev (same ld).
+ *   grad_dev [2][dims] f32 (gamma's row, beta's row), overwritten: the gradient
+ *            as the MEAN over the batch, FcLayer's convention (rowMeans,
+ *            layer/FcLayer.java:103-106).  NULL: added to the store's pending gradient
+ *            of "ln<i>.*" (KVStore.sum) for ps_ln_update / ps_dense_update. */
+int ps_ln_backward(ps_store_t *s, int layer, int type, const void *x_dev, int64_t ldx, const float *stats_dev,
+                   const void *dy_dev, int64_t lddy, int B, const void *skip_dev, int64_t ldskip,
+                   void *dx_dev, int64_t lddx, float *grad_dev);
+/* The pending sum of "ln<i>.weights" / ".bias" and its count (ps_fc_pending_grad's twin). */
+int ps_ln_pending_grad(ps_store_t *s, int layer, int bias, float *out, int cap, int *count);
+/* KVStore.update(Map) + clear for "ln<layer>.*": g = pending sum / count, every tensor's own
+ * updater.  globalStep++.  PS_MISSING without a pending gradient.  (ps_dense_update(s, -1)
+ * does it for every FC layer and every normalisation with a pending gradient.) */
+int ps_ln_update(ps_store_t *s, int layer);
+/* z = x W + b, y = act(z) + r of "fc<layer>" for x_dev [B][in].  r_dev [B][out] or
+ * NULL; z_dev [B][out] or NULL: the pre-activation, which ps_fc_res_backward
+ * needs unless act is NONE.  y_dev may be r_dev (same ld). */
+int ps_fc_res_forward(ps_store_t *s, int layer, int type, int act, const void *x_dev, int64_t ldx, int B,
+                      const void *r_dev, int64_t ldr, void *z_dev, int64_t ldz, void *y_dev, int64_t ldy);
+/* dz = dy act'(z) (z_dev may be NULL with PS_ACT_NONE), then
+ *   dx_dev   (NULL: not wanted) = skip + dz W^T; skip_dev [B][in] or NULL; dx_dev
+ *            may be skip_dev (same ld).  r's own gradient is dy itself.
+ *   grad_dev [in + 1][out] f32, overwritten: x^T dz / B, and in row `in` the
+ *            bias's, dz's mean.  NULL: added to the pending gradient of "fc<i>.*",
+ *            the one ps_fc_backward adds to. */
+int ps_fc_res_backward(ps_store_t *s, int layer, int type, int act, const void *x_dev, int64_t ldx,
+                       const void *z_dev, int64_t ldz, const void *dy_dev, int64_t lddy, int B,
+                       const void *skip_dev, int64_t ldskip, void *dx_dev, int64_t lddx, float *grad_dev);
 /* EmbeddingLayer.backward (layer/EmbeddingLayer.java:59-69) =
  * EmbeddingField.backward of every field (layer/EmbeddingField.java:86-104),
  * run TWICE per step by the reference (grad_mode

@@ -156,6 +156,18 @@ class KVStore:
     def create_fc(self, layer, in_dims, out_dims):
         N.check(N.lib().ps_store_create_fc(self.h, layer, in_dims, out_dims))
 
+    def create_ln(self, layer, dims):
+        """"ln<layer>.weights" (ones) / "ln<layer>.bias" (zeros): a layer normalisation's gamma and beta."""
+        N.check(N.lib().ps_store_create_ln(self.h, layer, dims))
+
+    def set_stream(self, stream):
+        """Adopt a HIP stream (its handle, e.g. torch.cuda.current_stream().cuda_stream) for everything this store enqueues."""
+        N.check(N.lib().ps_store_set_stream(self.h, stream))
+
+    def dense_update(self, layer=-1):
+        """KVStore.update(Map) + clear for the pending gradients of the dense tensors (layer < 0: every FC layer and normalisation)."""
+        N.check(N.lib().ps_dense_update(self.h, layer))
+
     def set_updater(self, key, updater):
         N.check(N.lib().ps_store_set_updater(self.h, key.encode(), C.byref(updater._s)))
 
@@ -484,6 +496,146 @@ class WideDeepNN(_Model):
         m._updater["wide.weights"] = ftrl
         m._updater["wide.bias"] = ftrl
         return m
+
+
+# ---------------------------------------------------------------------------
+# the residual tower: layer normalisation, FC with bias, activation and residual (ps_ln_*, ps_fc_res_*)
+# ---------------------------------------------------------------------------
+_TYPES = {}          # a tensor's dtype -> PS_T_*
+
+
+def _mat(t, name, B=None, width=None, like=None):
+    """(pointer, row stride) of a [B][width] device tensor (torch's, or anything with its attributes): checked, never copied."""
+    if t.dim() != 2 or (width is not None and t.shape[1] != width) or (B is not None and t.shape[0] != B):
+        raise N.PsError(N.PS_E_BAD_ARG, "%s: shape %s, wanted [%s][%s]" % (name, tuple(t.shape), "B" if B is None else B, width))
+    ld, inner = t.stride()
+    if inner != 1 and t.shape[1] > 1:
+        raise N.PsError(N.PS_E_BAD_ARG, "%s: the columns of a row must be neighbours (stride %d)" % (name, inner))
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise N.PsError(N.PS_E_BAD_ARG, "%s: %s on %s, wanted %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
+    if t.shape[0] <= 1:
+        ld = t.shape[1]                                # one row: its stride says nothing
+    return t.data_ptr(), ld
+
+
+def _f32(t, name, shape, like):
+    if tuple(t.shape) != shape or not t.is_contiguous() or t.device != like.device or str(t.dtype) != "torch.float32":
+        raise N.PsError(N.PS_E_BAD_ARG, "%s: wanted a contiguous float32 tensor of shape %s on %s" % (name, shape, like.device))
+    return t.data_ptr()
+
+
+class _TowerLayer:
+    def __init__(self, store, layer):
+        self.store, self.layer = store, layer
+
+    def _type(self, x):
+        t = _TYPES.get(x.dtype)
+        if t is None:
+            t = {"torch.float32": N.PS_T_F32, "torch.bfloat16": N.PS_T_BF16, "torch.float16": N.PS_T_F16}.get(str(x.dtype))
+            if t is None:
+                raise N.PsError(N.PS_E_BAD_ARG, "activations are float32, bfloat16 or float16, not %s" % x.dtype)
+            _TYPES[x.dtype] = t
+        if x.device.type != "cuda" or x.device.index != self.store.device:
+            raise N.PsError(N.PS_E_BAD_ARG, "x is on %s, the store on device %d" % (x.device, self.store.device))
+        return t
+
+    def _pending(self, fn, bias, shape):
+        out = np.empty(shape, np.float32)
+        n = C.c_int()
+        rc = fn(self.store.h, self.layer, int(bias), _fp(out), out.size, C.byref(n))
+        if rc == N.PS_MISSING and n.value == 0:
+            return None, 0
+        N.check(rc)
+        return out, n.value
+
+
+class LnLayer(_TowerLayer):
+    """Layer normalisation over the rows of a [B][dims] device tensor, "ln<layer>.*" of the store.  Tensors are torch's (float32,
+    bfloat16 or float16; rows may be strided), on the store's device and ready on the store's stream (KVStore.set_stream)."""
+
+    def __init__(self, store, layer, dims, eps=1e-5):
+        super().__init__(store, layer)
+        self.dims, self.eps = dims, eps
+        store.create_ln(layer, dims)
+
+    def forward(self, x, y=None, stats=None):
+        """y = (x - mean) / sqrt(var + eps) * gamma + beta; stats [B][2] float32 (filled): what backward needs."""
+        ty = self._type(x)
+        xp, ldx = _mat(x, "x", None, self.dims)
+        B = x.shape[0]
+        if y is None:
+            y = x.new_empty((B, self.dims))
+        yp, ldy = _mat(y, "y", B, self.dims, x)
+        sp = None if stats is None else _f32(stats, "stats", (B, 2), x)
+        N.check(N.lib().ps_ln_forward(self.store.h, self.layer, ty, xp, ldx, B, self.eps, yp, ldy, sp))
+        return y
+
+    def backward(self, x, stats, dy, skip=None, dx=None, grad=None, want_dx=True):
+        """dx (+ skip: the gradient that came round the normalisation).  grad [2][dims] float32: the mean gradients of gamma and
+        beta, overwritten; None: added to the store's pending gradient (KVStore.dense_update / update)."""
+        ty = self._type(x)
+        xp, ldx = _mat(x, "x", None, self.dims)
+        B = x.shape[0]
+        dyp, lddy = _mat(dy, "dy", B, self.dims, x)
+        kp, ldk = (None, 0) if skip is None else _mat(skip, "skip", B, self.dims, x)
+        if dx is None and want_dx:
+            dx = x.new_empty((B, self.dims))
+        dxp, lddx = (None, 0) if dx is None else _mat(dx, "dx", B, self.dims, x)
+        gp = None if grad is None else _f32(grad, "grad", (2, self.dims), x)
+        N.check(N.lib().ps_ln_backward(self.store.h, self.layer, ty, xp, ldx, _f32(stats, "stats", (B, 2), x), dyp, lddy, B, kp, ldk, dxp, lddx, gp))
+        return dx
+
+    def pending_grad(self, bias=False):
+        """(pending sum [dims], its count); (None, 0) without one"""
+        return self._pending(N.lib().ps_ln_pending_grad, bias, (self.dims,))
+
+    def update(self):
+        N.check(N.lib().ps_ln_update(self.store.h, self.layer))
+
+
+class FcResLayer(_TowerLayer):
+    """y = act(x W + b) + res over [B][in_dims] device tensors, "fc<layer>.*" of the store (the parameters FcLayer trains: float32;
+    16-bit activations multiply weights rounded to their type).  act: PS_ACT_NONE / RELU / GELU / SILU."""
+
+    def __init__(self, store, layer, in_dims, out_dims, act=N.PS_ACT_NONE):
+        super().__init__(store, layer)
+        self.in_dims, self.out_dims, self.act = in_dims, out_dims, act
+        store.create_fc(layer, in_dims, out_dims)
+
+    def forward(self, x, res=None, z=None, y=None):
+        """z [B][out_dims] (filled): the pre-activation, which backward needs unless act is NONE."""
+        ty = self._type(x)
+        xp, ldx = _mat(x, "x", None, self.in_dims)
+        B = x.shape[0]
+        if y is None:
+            y = x.new_empty((B, self.out_dims))
+        rp, ldr = (None, 0) if res is None else _mat(res, "res", B, self.out_dims, x)
+        zp, ldz = (None, 0) if z is None else _mat(z, "z", B, self.out_dims, x)
+        yp, ldy = _mat(y, "y", B, self.out_dims, x)
+        N.check(N.lib().ps_fc_res_forward(self.store.h, self.layer, ty, self.act, xp, ldx, B, rp, ldr, zp, ldz, yp, ldy))
+        return y
+
+    def backward(self, x, z, dy, skip=None, dx=None, grad=None, want_dx=True):
+        """dx = skip + (dy act'(z)) W^T.  grad [in_dims + 1][out_dims] float32: the mean gradients of W and, in the last row, b,
+        overwritten; None: added to the store's pending gradient.  res's own gradient is dy."""
+        ty = self._type(x)
+        xp, ldx = _mat(x, "x", None, self.in_dims)
+        B = x.shape[0]
+        zp, ldz = (None, 0) if z is None else _mat(z, "z", B, self.out_dims, x)
+        dyp, lddy = _mat(dy, "dy", B, self.out_dims, x)
+        kp, ldk = (None, 0) if skip is None else _mat(skip, "skip", B, self.in_dims, x)
+        if dx is None and want_dx:
+            dx = x.new_empty((B, self.in_dims))
+        dxp, lddx = (None, 0) if dx is None else _mat(dx, "dx", B, self.in_dims, x)
+        gp = None if grad is None else _f32(grad, "grad", (self.in_dims + 1, self.out_dims), x)
+        N.check(N.lib().ps_fc_res_backward(self.store.h, self.layer, ty, self.act, xp, ldx, zp, ldz, dyp, lddy, B, kp, ldk, dxp, lddx, gp))
+        return dx
+
+    def pending_grad(self, bias=False):
+        return self._pending(N.lib().ps_fc_pending_grad, bias, (self.out_dims,) if bias else (self.in_dims, self.out_dims))
+
+    def update(self):
+        self.store.dense_update(self.layer)
 
 
 class Trainer:

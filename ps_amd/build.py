@@ -15,7 +15,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libps_amd.so")
-SOURCES = ["kernels_sort.hip", "kernels_gemm.hip", "kernels_emb.hip", "ps_store.hip", "ps_model.hip", "ps_ops.hip", "ps_layer_ops.hip", "ps_shard.hip", "ps_ingest.hip", "ps_eval.hip", "ps_ckpt.hip", "ps_comm.hip", "ps_keyed.hip"]
+SOURCES = ["kernels_sort.hip", "kernels_gemm.hip", "kernels_emb.hip", "ps_store.hip", "ps_model.hip", "ps_ops.hip", "ps_layer_ops.hip", "ps_shard.hip", "ps_ingest.hip", "ps_eval.hip", "ps_ckpt.hip", "ps_comm.hip", "ps_keyed.hip",
+           "kernels_ln.hip", "kernels_fcres.hip", "ps_tower.hip"]
 # -ffp-contract=off: the reference (JVM) rounds every float op separately;
 # the updater / reduce kernels must too, to stay bit-exact with the oracle.
 # -packed-fp32-ops: no packed f32 instructions (hipcc makes them from ordinary float code); some of their forms have given wrong

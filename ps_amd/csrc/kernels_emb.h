@@ -232,6 +232,7 @@ int launch_init_emb(float *W, int64_t rows, int D, uint64_t seed, uint64_t table
                     int64_t id_first, int64_t id_stride, const uint32_t *ids_dev /* NULL: id_first + r*id_stride */, hipStream_t st);
 int launch_init_dense(float *W, float *Wt, int K, int N, int ldw, int ldwt, uint64_t seed,
                       uint64_t table_w, float scale_w, uint64_t table_b, float scale_b, hipStream_t st);
+int launch_transpose_w(const float *W, float *Wt, int Kpad, int ldw, int N, hipStream_t st);      // Wt = W'^T (after a load)
 int launch_fill(float *p, int64_t n, float v, hipStream_t st);
 int launch_fill_col(float *p, int rows, int ld, int col, float v, hipStream_t st);
 int launch_rows_copy(float *table, int64_t row_stride, int64_t col_off, const int64_t *rows_idx_dev,

@@ -1,0 +1,363 @@
+// kernels_fcres.hip -- the FC layer with bias, activation and residual in its epilogue, and its gradients (gfx950 matrix cores).
+//
+//   forward    z = x W + b,  y = act(z) + r
+//   backward   dz = dy act'(z),  dx = skip + dz W^T,  dW = x^T dz / B,  db = sum dz / B
+//
+// Three products: x W and dz W^T are both "NT" (rows of activations times rows of a weight matrix, both contiguous along the sum: the
+// store keeps W and its transpose), x^T dz is "TN" (the sum runs over the batch, across the rows of both).  Activations are f32, bf16
+// or f16; weights are f32 in the store and are rounded to the activations' type on their way into LDS; sums are f32.
+#include "kernels_tower.h"
+
+namespace {
+
+template <typename T> struct Mma;      // one matrix instruction: NI x MI results, KS of the sum
+template <> struct Mma<__bf16> {
+    typedef bf16x8 frag; typedef f32x4 acc;
+    static constexpr int TILE = 16, BK = 64;
+    static __device__ __forceinline__ acc mma(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<_Float16> {
+    typedef f16x8 frag; typedef f32x4 acc;
+    static constexpr int TILE = 16, BK = 64;
+    static __device__ __forceinline__ acc mma(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<float> {        // a fragment holds 4 steps of 2: the lanes' halves take k = 8 i + 4 h + j, the same for both operands
+    typedef f32x4 frag; typedef f32x16 acc;
+    static constexpr int TILE = 32, BK = 32;
+    static __device__ __forceinline__ acc mma(frag a, frag b, acc c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+__device__ __forceinline__ float act_apply(float z, int act) {
+    if (act == PS_ACT_RELU) return z < 0.f ? 0.f : z;      // (a NaN stays one)
+    if (act == PS_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if (act == PS_ACT_SILU) return z / (1.f + expf(-z));
+    return z;
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == PS_ACT_GELU) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    const float p = 1.f / (1.f + expf(-z));
+    return p * (1.f + z * (1.f - p));
+}
+
+// workgroup -> tile so that an XCD (workgroup id mod 8) owns a contiguous range of tiles: its L2 then serves the tiles' shared rows
+__device__ __forceinline__ int xcd_tile(int id, int n) {
+    const int q = n >> 3, r = n & 7, x = id & 7, i = id >> 3;
+    return x * q + (x < r ? x : r) + i;
+}
+
+// 8 (4) weights of one row as 16 bytes of the activations' type
+template <typename T> __device__ __forceinline__ void load_w(Chunk<T> &o, const float *row, int c, int n) {
+    if constexpr (sizeof(T) == 4) {
+        o.load(row, c, n);
+    } else {
+        float w[8];
+        if (c + 8 <= n) {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(row + c), hi = *reinterpret_cast<const f32x4 *>(row + c + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { w[j] = lo[j]; w[4 + j] = hi[j]; }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = c + j < n ? row[c + j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o.e[j] = (T)w[j];
+    }
+}
+
+// One BM x BN tile of the output per workgroup of 4 waves (2 x 2).  LDS rows are 128 bytes of the sum's axis (BK elements), 16-byte
+// pieces exchanged by the row's low bits so that the fragment reads of 8 neighbouring rows touch all banks once.  The next step's
+// pieces travel in registers while this step multiplies; two LDS buffers, one barrier a step.
+// The product is formed transposed (weights as the first operand): a lane then holds 4 neighbouring columns of one row of y.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256) void k_fc_nt(FcNtArgs a, int tiles_n) {
+    typedef Mma<T> X;
+    typedef typename X::frag frag;
+    constexpr int CN = Chunk<T>::N, BK = X::BK, TILE = X::TILE, FM = BM / 2 / TILE, FN = BN / 2 / TILE, PA = BM * 8 / 256, PB = BN * 8 / 256;
+    __shared__ u32x4 sA[2][BM * 8], sB[2][BN * 8];
+    const int tile = xcd_tile(blockIdx.x, gridDim.x);
+    const int64_t m0 = (int64_t)(tile / tiles_n) * BM;
+    const int n0 = (tile % tiles_n) * BN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+    const T *pa[PA];
+    const float *pb[PB];
+    int dst_a[PA], dst_b[PB];
+    const int ch = tid & 7;
+#pragma unroll
+    for (int i = 0; i < PA; ++i) {
+        const int row = (tid >> 3) + i * 32;
+        const int64_t m = m0 + row < a.M ? m0 + row : a.M - 1;      // rows behind the last: any row, their results go nowhere
+        pa[i] = (const T *)a.A + m * a.lda;
+        dst_a[i] = row * 8 + (ch ^ (row & 7));
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+        const int row = (tid >> 3) + i * 32, n = n0 + row < a.N ? n0 + row : a.N - 1;
+        pb[i] = a.W + (size_t)n * a.ldw;
+        dst_b[i] = row * 8 + (ch ^ (row & 7));
+    }
+    Chunk<T> ra[PA], rb[PB];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < PA; ++i) ra[i].load(pa[i], k0 + ch * CN, a.K);
+#pragma unroll
+        for (int i = 0; i < PB; ++i) load_w<T>(rb[i], pb[i], k0 + ch * CN, a.K);
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < PA; ++i) sA[buf][dst_a[i]] = ra[i].u;
+#pragma unroll
+        for (int i = 0; i < PB; ++i) sB[buf][dst_b[i]] = rb[i].u;
+    };
+    typename X::acc acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+            for (int e = 0; e < (int)(sizeof(acc[0][0]) / 4); ++e) acc[i][j][e] = 0.f;
+    const int lr = lane % TILE, lg = lane / TILE;
+    constexpr int KS = 8 / (64 / TILE);          // fragment steps per LDS row
+    fetch(0);
+    put(0);
+    __syncthreads();
+    const int steps = (a.K + BK - 1) / BK;
+    for (int s = 0; s < steps; ++s) {
+        const int buf = s & 1;
+        if (s + 1 < steps) fetch((s + 1) * BK);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            frag fa[FM], fb[FN];
+            const int c = ks * (64 / TILE) + lg;
+#pragma unroll
+            for (int j = 0; j < FM; ++j) { const int r = wm + j * TILE + lr; fa[j] = *reinterpret_cast<const frag *>(&sA[buf][r * 8 + (c ^ (r & 7))]); }
+#pragma unroll
+            for (int i = 0; i < FN; ++i) { const int r = wn + i * TILE + lr; fb[i] = *reinterpret_cast<const frag *>(&sB[buf][r * 8 + (c ^ (r & 7))]); }
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FM; ++j) acc[i][j] = X::mma(fb[i], fa[j], acc[i][j]);
+        }
+        if (s + 1 < steps) put(buf ^ 1);
+        __syncthreads();
+    }
+    // epilogue: groups of 4 neighbouring columns of one row
+    constexpr int GR = (int)(sizeof(acc[0][0]) / 16);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int64_t m = m0 + wm + j * TILE + lr;
+        if (m >= a.M) continue;
+        T *y = (T *)a.Y + m * a.ldy, *zr = (T *)a.Z + m * a.ldz;
+        const T *rr = (const T *)a.R + m * a.ldr;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int q = 0; q < GR; ++q) {
+                const int n = n0 + wn + i * TILE + q * 8 + lg * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (n + e >= a.N) continue;
+                    float v = acc[i][j][q * 4 + e];
+                    if (a.bias) v += a.bias[n + e];
+                    if (a.Z) zr[n + e] = (T)v;
+                    v = act_apply(v, a.act);
+                    if (a.R) v += (float)rr[n + e];
+                    y[n + e] = (T)v;
+                }
+            }
+    }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T *dy, int64_t lddy, const T *z, int64_t ldz, T *dz, int64_t lddz, int M, int N, int act) {
+    const int64_t per = (N + Chunk<T>::N - 1) / Chunk<T>::N, total = per * M;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / per;
+        const int c = (int)(i % per) * Chunk<T>::N;
+        Chunk<T> d, v;
+        d.load(dy + m * lddy, c, N);
+        v.load(z + m * ldz, c, N);
+#pragma unroll
+        for (int j = 0; j < Chunk<T>::N; ++j) {
+            const float zz = (float)v.e[j];
+            d.e[j] = act == PS_ACT_RELU ? (zz > 0.f ? d.e[j] : (T)0.f) : (T)((float)d.e[j] * act_slope(zz, act));
+        }
+        d.store(dz + m * lddz, c, N);
+    }
+}
+
+// One 128 x 128 tile of x^T dz over one part of the batch.  LDS holds the rows as they lie in memory; 16-bit fragments need 8 values
+// down a column, which the transposing LDS read delivers (16 lanes read 4 rows x 16 columns and get a column's 4 rows each).  The order
+// of the sum inside a step is the same for both operands and otherwise free.  32-byte pieces are exchanged by the row's low bits: the
+// 4 rows of a transposing read lie in 4 different bank groups.  The workgroups of the first row of tiles also multiply dz by a
+// fragment of ones: db, row K of the slab.
+template <typename T>
+__global__ __launch_bounds__(256) void k_fc_tn(FcTnArgs a, int tiles_n, int tiles) {
+    typedef Mma<T> X;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int CN = Chunk<T>::N, BT = 128, ROWS = F32 ? 32 : 64, PER = BT / CN, P = ROWS * PER / 256, TILE = X::TILE, FK = BT / 2 / TILE, FN = BT / 2 / TILE;
+    __shared__ u32x4 sX[2][ROWS * PER], sD[2][ROWS * PER];
+    const int id = xcd_tile(blockIdx.x, gridDim.x);
+    const int split = id / tiles, tile = id % tiles, k0 = (tile / tiles_n) * BT, n0 = (tile % tiles_n) * BT;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = (wave >> 1) * (BT / 2), wn = (wave & 1) * (BT / 2);
+    // this part's rows: whole steps, dealt evenly
+    const int64_t all = ((int64_t)a.M + ROWS - 1) / ROWS;
+    const int64_t s_lo = all * split / a.nsplit, s_hi = all * (split + 1) / a.nsplit;
+    Chunk<T> rx[P], rd[P];
+    int dst[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int q = tid + i * 256, row = q / PER, c = q % PER;
+        dst[i] = row * PER + (F32 ? c : c ^ ((row & 7) << 1));
+    }
+    auto fetch = [&](int64_t s) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int q = tid + i * 256, row = q / PER, c = (q % PER) * CN;
+            const int64_t m = s * ROWS + row;
+            if (m < a.M) {
+                rx[i].load((const T *)a.X + m * a.ldx, k0 + c, a.K);
+                rd[i].load((const T *)a.D + m * a.ldd, n0 + c, a.N);
+            } else {
+                rx[i].zero(); rd[i].zero();
+            }
+        }
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) { sX[buf][dst[i]] = rx[i].u; sD[buf][dst[i]] = rd[i].u; }
+    };
+    typename X::acc acc[FK][FN], accb[FN];
+    constexpr int AE = (int)(sizeof(accb[0]) / 4);
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < AE; ++e) {
+            accb[j][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < FK; ++i) acc[i][j][e] = 0.f;
+        }
+    typename X::frag ones;
+#pragma unroll
+    for (int j = 0; j < CN; ++j) ones[j] = (T)1.f;
+    const bool do_bias = k0 == 0 && wk == 0;
+    const int lr = lane % TILE, lg = lane / TILE;
+    if (s_lo < s_hi) { fetch(s_lo); put(0); }
+    __syncthreads();
+    for (int64_t s = s_lo; s < s_hi; ++s) {
+        const int buf = (int)(s - s_lo) & 1;
+        if (s + 1 < s_hi) fetch(s + 1);
+#pragma unroll
+        for (int ks = 0; ks < (F32 ? 4 : 2); ++ks) {
+            typename X::frag fk[FK], fn[FN];
+            if constexpr (F32) {
+                const float *lx = reinterpret_cast<const float *>(sX[buf]), *ld = reinterpret_cast<const float *>(sD[buf]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = ks * 8 + e * 2 + lg;
+#pragma unroll
+                    for (int i = 0; i < FK; ++i) fk[i][e] = lx[row * BT + wk + i * TILE + lr];
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) fn[j][e] = ld[row * BT + wn + j * TILE + lr];
+                }
+            } else {
+                typedef __attribute__((address_space(3))) s16x4 lds4;
+                union { typename X::frag f; s16x4 h[2]; } u;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const u32x4 *base = w ? sD[buf] : sX[buf];
+#pragma unroll
+                    for (int i = 0; i < (FK > FN ? FK : FN); ++i) {
+                        const int col = (w ? wn : wk) + i * 16;                  // 32-byte piece col / 16
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int row = ks * 32 + h * 16 + lg * 4 + (lr >> 2);
+                            const short *p = reinterpret_cast<const short *>(base) + row * BT + ((col >> 4) ^ (row & 7)) * 16 + (lr & 3) * 4;
+                            u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
+                        }
+                        if (w) fn[i] = u.f; else fk[i] = u.f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < FK; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = X::mma(fk[i], fn[j], acc[i][j]);
+            if (do_bias) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) accb[j] = X::mma(ones, fn[j], accb[j]);
+            }
+        }
+        if (s + 1 < s_hi) put(buf ^ 1);
+        __syncthreads();
+    }
+    float *part = a.part + (size_t)split * (size_t)(a.K + 1) * a.N;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + wn + j * TILE + lr;
+        if (n >= a.N) continue;
+#pragma unroll
+        for (int i = 0; i < FK; ++i)
+#pragma unroll
+            for (int e = 0; e < AE; ++e) {
+                const int k = k0 + wk + i * TILE + (e >> 2) * 8 + lg * 4 + (e & 3);
+                if (k < a.K) part[(size_t)k * a.N + n] = acc[i][j][e];
+            }
+        if (do_bias && lg == 0) part[(size_t)a.K * a.N + n] = accb[j][0];
+    }
+}
+
+int grid_ok(int64_t blocks) {
+    return blocks * 256 < (1ll << 32) ? PS_OK : ps_set_err(PS_E_UNSUPPORTED, "the batch needs more workgroups than one launch has");
+}
+
+template <typename T, int BM, int BN> int nt_go(const FcNtArgs &a, hipStream_t st) {
+    const int tiles_n = cdiv(a.N, BN);
+    const int64_t blocks = (int64_t)tiles_n * cdiv(a.M, BM);
+    PSCHK(grid_ok(blocks));
+    hipLaunchKernelGGL((k_fc_nt<T, BM, BN>), dim3((unsigned)blocks), dim3(256), 0, st, a, tiles_n);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
+}
+template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
+    if ((int64_t)cdiv(a.M, 128) * cdiv(a.N, 128) >= 256) return nt_go<T, 128, 128>(a, st);
+    return nt_go<T, 64, 64>(a, st);
+}
+template <typename T> int tn_t(const FcTnArgs &a, hipStream_t st) {
+    const int tiles_n = cdiv(a.N, 128), tiles = tiles_n * cdiv(a.K, 128);
+    const int64_t blocks = (int64_t)tiles * a.nsplit;
+    PSCHK(grid_ok(blocks));
+    hipLaunchKernelGGL((k_fc_tn<T>), dim3((unsigned)blocks), dim3(256), 0, st, a, tiles_n, tiles);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
+}
+template <typename T>
+int ag_t(int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st) {
+    const int64_t blocks = ((int64_t)cdiv(N, Chunk<T>::N) * M + 255) / 256;
+    hipLaunchKernelGGL((k_act_grad<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, (const T *)dy, lddy, (const T *)z, ldz,
+                       (T *)dz, lddz, M, N, act);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
+}
+
+}  // namespace
+
+int launch_fc_nt(int type, const FcNtArgs &a, hipStream_t st) {
+    return type == PS_T_F32 ? nt_t<float>(a, st) : type == PS_T_BF16 ? nt_t<__bf16>(a, st) : nt_t<_Float16>(a, st);
+}
+int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st) {
+    return type == PS_T_F32    ? ag_t<float>(act, dy, lddy, z, ldz, dz, lddz, M, N, st)
+           : type == PS_T_BF16 ? ag_t<__bf16>(act, dy, lddy, z, ldz, dz, lddz, M, N, st)
+                               : ag_t<_Float16>(act, dy, lddy, z, ldz, dz, lddz, M, N, st);
+}
+int fc_tn_splits(int type, int M, int K, int N) {
+    const int64_t tiles = (int64_t)cdiv(N, 128) * cdiv(K, 128), steps = cdiv(M, type == PS_T_F32 ? 32 : 64);
+    int64_t s = (512 + tiles - 1) / tiles;               // two workgroups for each of the 256 CUs
+    if (s > steps / 4) s = steps / 4;                    // and no part shorter than four steps
+    return (int)(s < 1 ? 1 : s);
+}
+int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st) {
+    return type == PS_T_F32 ? tn_t<float>(a, st) : type == PS_T_BF16 ? tn_t<__bf16>(a, st) : tn_t<_Float16>(a, st);
+}

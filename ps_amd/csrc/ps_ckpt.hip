@@ -7,7 +7,7 @@
 //   magic "PSAMDCK1", header (device-independent ints), then sections in fixed order:
 //     embedding W [total_rows][D], state [total_rows][2][D] (if any)
 //     wide W [rows], state [rows][2], touched [rows] (u8), bias[1], bias_state[2]      (if a wide table exists)
-//     per FC layer: W' [Kpad][ldw], S1, S2                                            (Wt is rebuilt on load)
+//     per FC layer, then per normalisation: W' [Kpad][ldw], S1, S2                    (Wt is rebuilt on load)
 //     the updaters registered on the store (name -> parameters), globalStep
 //
 // One file per shard (rank): every rank saves its own rows, the replicated tensors are identical on all ranks.
@@ -66,8 +66,23 @@ struct IO {
     }
 };
 
+// the dense tensors of a store, FC layers first, with the number the file knows each by (a normalisation's starts at kLnBase: a
+// file without any is what it was before there were normalisations)
+const int32_t kLnBase = 1 << 16;
+template <typename F> void each_dense(ps_store *s, F fn) {
+    for (size_t l = 0; l < s->fc.size(); ++l)
+        if (s->fc[l].present) fn((int32_t)l, s->fc[l]);
+    for (size_t l = 0; l < s->ln.size(); ++l)
+        if (s->ln[l].present) fn(kLnBase + (int32_t)l, s->ln[l]);
+}
+FcParams *dense_by_number(ps_store *s, int32_t d) {
+    std::vector<FcParams> &v = d >= kLnBase ? s->ln : s->fc;
+    const int32_t l = d >= kLnBase ? d - kLnBase : d;
+    return l >= 0 && l < (int32_t)v.size() && v[l].present ? &v[l] : nullptr;
+}
+
 // bytes sections() moves for this store's geometry (what a complete file holds after its header)
-size_t section_bytes(const ps_store *s) {
+size_t section_bytes(ps_store *s) {
     size_t n = 0;
     const EmbTables &e = s->emb;
     if (e.W) {
@@ -76,8 +91,7 @@ size_t section_bytes(const ps_store *s) {
     }
     const WideTable &w = s->wide;
     if (w.W) n += sizeof(float) * (size_t)w.rows * 3 + (size_t)w.rows + sizeof(float) * 3;
-    for (auto &f : s->fc)
-        if (f.present) n += 3 * sizeof(float) * (size_t)f.Kpad * f.ldw;
+    each_dense(s, [&](int32_t, FcParams &f) { n += 3 * sizeof(float) * (size_t)f.Kpad * f.ldw; });
     return n;
 }
 
@@ -98,20 +112,17 @@ int sections(IO &io) {
         PSCHK(io.dev(w.bias, sizeof(float)));
         PSCHK(io.dev(w.bias_state, sizeof(float) * 2));
     }
-    for (auto &f : s->fc) {
-        if (!f.present) continue;
+    int rc = PS_OK;
+    each_dense(s, [&](int32_t, FcParams &f) {
         const size_t n = sizeof(float) * (size_t)f.Kpad * f.ldw;
-        PSCHK(io.dev(f.W, n));
-        PSCHK(io.dev(f.S1, n));
-        PSCHK(io.dev(f.S2, n));
-    }
-    return PS_OK;
+        for (float *p : {f.W, f.S1, f.S2})
+            if (rc == PS_OK) rc = io.dev(p, n);
+    });
+    return rc;
 }
 
 }  // namespace
 
-// defined in kernels_emb.hip: Wt = W'^T after a load
-int launch_transpose_w(const float *W, float *Wt, int Kpad, int ldw, int N, hipStream_t st);
 
 extern "C" int ps_store_save(ps_store_t *s, const char *path) {
     if (!s || !path) return ps_set_err(PS_E_BAD_ARG, "null argument");
@@ -131,16 +142,15 @@ extern "C" int ps_store_save(ps_store_t *s, const char *path) {
     h.F = s->emb.F; h.D = s->emb.D; h.state_slots = s->emb.state ? 2 : 0;
     h.shard = s->emb.shard; h.nshards = s->emb.nshards; h.route_mode = s->emb.route_mode;
     h.nfc = 0;
-    for (auto &f : s->fc) h.nfc += f.present ? 1 : 0;
+    each_dense(s, [&](int32_t, FcParams &) { h.nfc++; });
     h.nupd = (int32_t)s->updaters.size();
     io.raw((void *)kMagic, 8);
     io.raw(&h, sizeof h);
     for (int f = 0; f < s->emb.F; ++f) { int64_t v = s->emb.rows[f]; io.raw(&v, 8); }
-    for (size_t l = 0; l < s->fc.size(); ++l) {
-        if (!s->fc[l].present) continue;
-        int32_t d[3] = {(int32_t)l, s->fc[l].K, s->fc[l].N};
+    each_dense(s, [&](int32_t l, FcParams &f) {
+        int32_t d[3] = {l, f.K, f.N};
         io.raw(d, sizeof d);
-    }
+    });
     for (auto &kv : s->updaters) {
         int32_t n = (int32_t)kv.first.size();
         io.raw(&n, 4);
@@ -185,13 +195,13 @@ extern "C" int ps_store_load(ps_store_t *s, const char *path) {
         if (!io.ok || v != s->emb.rows[f]) return fail(PS_E_BAD_ARG, "a field's vocabulary differs from this store");
     }
     int nfc_here = 0;
-    for (auto &f : s->fc) nfc_here += f.present ? 1 : 0;
-    if (h.nfc != nfc_here) return fail(PS_E_BAD_ARG, "number of FC layers differs from this store");
+    each_dense(s, [&](int32_t, FcParams &) { nfc_here++; });
+    if (h.nfc != nfc_here) return fail(PS_E_BAD_ARG, "number of FC layers (or normalisations) differs from this store");
     for (int i = 0; i < h.nfc; ++i) {
         int32_t d[3];
         io.raw(d, sizeof d);
-        if (!io.ok || d[0] < 0 || d[0] >= (int)s->fc.size() || !s->fc[d[0]].present || s->fc[d[0]].K != d[1] || s->fc[d[0]].N != d[2])
-            return fail(PS_E_BAD_ARG, "an FC layer's shape differs from this store");
+        const FcParams *f = io.ok ? dense_by_number(s, d[0]) : nullptr;
+        if (!f || f->K != d[1] || f->N != d[2]) return fail(PS_E_BAD_ARG, "an FC layer's (or a normalisation's) shape differs from this store");
     }
     std::map<std::string, ps_updater_t> upd;
     for (int i = 0; i < h.nupd; ++i) {
@@ -222,8 +232,11 @@ extern "C" int ps_store_load(ps_store_t *s, const char *path) {
     fclose(io.f);
     if (rc != PS_OK || !io.ok)
         return ps_set_err(rc != PS_OK ? rc : PS_E_HIP, "%s: read error while loading; the store now holds a MIX of old and new tensors -- reload or recreate it", path);
-    for (auto &f : s->fc)
-        if (f.present) { PSCHK(launch_transpose_w(f.W, f.Wt, f.Kpad, f.ldw, f.N, s->stream)); PSCHK(launch_pack_w(f.Wt, f.Wp, f.N, f.Kpad, s->stream)); }
+    each_dense(s, [&](int32_t, FcParams &f) {
+        if (rc == PS_OK) rc = launch_transpose_w(f.W, f.Wt, f.Kpad, f.ldw, f.N, s->stream);
+        if (rc == PS_OK) rc = launch_pack_w(f.Wt, f.Wp, f.N, f.Kpad, s->stream);
+    });
+    PSCHK(rc);
     HIPCHK(hipStreamSynchronize(s->stream));
     s->updaters = upd;
     s->global_step = h.global_step;

@@ -1,7 +1,8 @@
 // ps_keyed.hip -- the PS server's side of the reference's wire, by STRING KEY:
 //   PServer.push(key, gradient, isAsync, updaterKey)   net/PServer.java:164-195   (KVStore.sum)
 //   PServer.psUpdate()                                 net/PServer.java:197-214   (KVStore.update(updater, key) per pushed key)
-// for any key the store holds: "emF<f>.<id>.0", "wide.weights.<id>.0", "wide.bias", "fc<i>.weights", "fc<i>.bias".
+// for any key the store holds: "emF<f>.<id>.0", "wide.weights.<id>.0", "wide.bias", "fc<i>.weights", "fc<i>.bias",
+// "ln<i>.weights", "ln<i>.bias".
 // ps_store_push_update takes the messages of one BSP round (every worker's pushes, in arrival order) -- or, async,
 // the messages to apply one by one -- and runs sum / divi(count) / Updater.update on the device with the arithmetic of
 // the hot path's kernels: embedding rows through the stable-sort path of ps_shard_apply_push (mean over a key's pushes
@@ -23,6 +24,12 @@ struct DevBuf {            // scratch for one call (the facade is not a hot path
     int alloc(size_t bytes) { RtGuard g; HIPCHK(hipMalloc(&p, bytes ? bytes : 4)); return PS_OK; }
 };
 
+const int kLnBase = 1 << 16;
+std::string dense_name(const std::pair<int, int> &t) {
+    const bool ln = t.first >= kLnBase;
+    return (ln ? "ln" : "fc") + std::to_string(ln ? t.first - kLnBase : t.first) + (t.second ? ".bias" : ".weights");
+}
+
 }  // namespace
 
 // The number of floats a push / upsert of `key` must carry on THIS shard (PS_MISSING: a key the store does not hold).
@@ -41,8 +48,9 @@ extern "C" int ps_store_key_length(const ps_store_t *s, const char *key, int *le
         if (k.kind == 1 && (k.id < 0 || k.id >= s->wide.rows)) return ps_set_err(PS_MISSING, "%s out of range", key);
         *len_out = 1;
     } else {
-        if (k.idx < 0 || k.idx >= (int)s->fc.size() || !s->fc[k.idx].present) return ps_set_err(PS_MISSING, "%s absent", key);
-        *len_out = k.kind == 4 ? s->fc[k.idx].N : s->fc[k.idx].K * s->fc[k.idx].N;
+        const FcParams *p = store_dense(const_cast<ps_store_t *>(s), k);
+        if (!p) return ps_set_err(PS_MISSING, "%s absent", key);
+        *len_out = key_is_bias(k) ? p->N : p->K * p->N;
     }
     return PS_OK;
 }
@@ -63,7 +71,7 @@ extern "C" int ps_store_push_update(ps_store_t *s, int n, const char *const *key
     std::vector<uint32_t> rows;                                    // embedding rows: one list in arrival order, duplicates =
     std::vector<float> eg;                                         // several workers' pushes of one key
     std::map<int64_t, std::vector<int>> wide;                      // wide keys: ascending key, message order inside
-    std::map<std::pair<int, int>, std::vector<int>> dense;        // (layer, bias) -> messages
+    std::map<std::pair<int, int>, std::vector<int>> dense;        // (layer, bias; normalisations behind the FC layers) -> messages
     const int D = s->emb.D;
     for (int i = 0; i < n; ++i) {
         if (lens[i] < 0) return ps_set_err(PS_E_BAD_ARG, "message %d: negative length", i);
@@ -80,11 +88,11 @@ extern "C" int ps_store_push_update(ps_store_t *s, int n, const char *const *key
             if (pk[i].kind == 1 && (pk[i].id < 0 || pk[i].id >= s->wide.rows)) return ps_set_err(PS_MISSING, "%s out of range", keys[i]);
             wide[pk[i].kind == 2 ? s->wide.rows : pk[i].id].push_back(i);
         } else {
-            const int l = pk[i].idx;
-            if (l < 0 || l >= (int)s->fc.size() || !s->fc[l].present) return ps_set_err(PS_MISSING, "%s absent", keys[i]);
-            const int want = pk[i].kind == 4 ? s->fc[l].N : s->fc[l].K * s->fc[l].N;
+            const FcParams *p = store_dense(s, pk[i]);
+            if (!p) return ps_set_err(PS_MISSING, "%s absent", keys[i]);
+            const int want = key_is_bias(pk[i]) ? p->N : p->K * p->N;
             if (lens[i] != want) return ps_set_err(PS_E_BAD_ARG, "%s wants %d floats, got %d", keys[i], want, lens[i]);
-            dense[{l, pk[i].kind == 4 ? 1 : 0}].push_back(i);
+            dense[{pk[i].idx + (key_is_ln(pk[i]) ? kLnBase : 0), key_is_bias(pk[i]) ? 1 : 0}].push_back(i);
         }
     }
     {   // (updaters too: PServer.push answers 500 for an unknown updater before anything is summed)
@@ -96,9 +104,7 @@ extern "C" int ps_store_push_update(ps_store_t *s, int n, const char *const *key
         if (!rows.empty() && !s->emb.state && stateful) return ps_set_err(PS_MISSING, "no embedding tables with updater state");
         if (!wide.empty()) PSCHK(store_resolve_updater(s, "wide.weights", &u));
         for (auto &kv : dense) {
-            char name[64];
-            snprintf(name, sizeof name, "fc%d.%s", kv.first.first, kv.first.second ? "bias" : "weights");
-            PSCHK(store_resolve_updater(s, name, &u));
+            PSCHK(store_resolve_updater(s, dense_name(kv.first).c_str(), &u));
         }
     }
     // ---- pass 2: apply ----
@@ -143,8 +149,8 @@ extern "C" int ps_store_push_update(ps_store_t *s, int n, const char *const *key
     std::vector<DevBuf> slabs(dense.size());
     size_t di = 0;
     for (auto &kv : dense) {
-        const int l = kv.first.first, bias = kv.first.second;
-        FcParams &p = s->fc[l];
+        const int bias = kv.first.second;
+        FcParams &p = *store_dense(s, pk[kv.second[0]]);
         const size_t len = bias ? (size_t)p.N : (size_t)p.K * p.N;
         const int m = (int)kv.second.size();
         DevBuf &buf = slabs[di++];
@@ -152,9 +158,7 @@ extern "C" int ps_store_push_update(ps_store_t *s, int n, const char *const *key
         for (int j = 0; j < m; ++j)
             HIPCHK(hipMemcpyAsync((float *)buf.p + (size_t)j * len, grads[kv.second[j]], sizeof(float) * len, hipMemcpyHostToDevice, st));
         ps_updater_t u;
-        char name[64];
-        snprintf(name, sizeof name, "fc%d.%s", l, bias ? "bias" : "weights");
-        PSCHK(store_resolve_updater(s, name, &u));
+        PSCHK(store_resolve_updater(s, dense_name(kv.first).c_str(), &u));
         const int launches = is_async ? m : 1;
         for (int j = 0; j < launches; ++j) {
             DenseUpdArgs d;

@@ -131,30 +131,50 @@ extern "C" int ps_fc_pending_grad(ps_store_t *s, int layer, int bias, float *out
     return PS_OK;
 }
 
+// KVStore.update(Map): g = sum / sumCnt, updater by key (exact, prefix, "default"), then clear (:240-277)
+int store_apply_pending(ps_store *s, FcParams &p, const char *stem, int layer, bool *done) {
+    *done = false;
+    if (!p.present || !p.pending || p.pending_cnt == 0) return PS_OK;
+    char key[32];
+    snprintf(key, sizeof key, "%s%d.weights", stem, layer);
+    ps_updater_t u, ub;
+    PSCHK(store_resolve_updater(s, key, &u));
+    ub = u;
+    if (s->ln.data() <= &p && &p < s->ln.data() + s->ln.size()) {        // a normalisation's beta is a tensor of its own
+        snprintf(key, sizeof key, "%s%d.bias", stem, layer);
+        PSCHK(store_resolve_updater(s, key, &ub));
+    }
+    const bool split = memcmp(&u, &ub, sizeof u) != 0;
+    for (int part = 0; part < (split ? 2 : 1); ++part) {
+        DenseUpdArgs d;
+        memset(&d, 0, sizeof d);
+        d.nlayers = 1; d.B = 1; d.apply = 1; d.flat_grad = p.pending; d.flat_div = (float)p.pending_cnt;
+        d.upd = make_upd_params(part ? ub : u);
+        DenseLayer &L = d.L[0];
+        L.W = p.W; L.Wt = p.Wt; L.Wp = p.Wp; L.S1 = p.S1; L.S2 = p.S2; L.K = p.K; L.N = p.N; L.ldw = p.ldw; L.ldwt = p.Kpad;
+        if (split) { L.row_lo = part ? p.K : 0; L.row_cnt = part ? 1 : p.K; }
+        L.elem_begin = 0; L.elem_end = (int64_t)(p.K + 1) * p.N;
+        PSCHK(launch_dense_update(d, s->stream));
+    }
+    p.pending_cnt = 0;
+    *done = true;
+    return PS_OK;
+}
+
 extern "C" int ps_dense_update(ps_store_t *s, int layer) {
     RoctxRange roctx_range("ps_dense_update");
     if (!s) return ps_set_err(PS_E_BAD_ARG, "store is NULL");
     PSCHK(store_enter(s));
     int done = 0;
+    bool one = false;
     for (int l = 0; l < (int)s->fc.size(); ++l) {
         if (layer >= 0 && l != layer) continue;
-        FcParams &p = s->fc[l];
-        if (!p.present || !p.pending || p.pending_cnt == 0) continue;
-        // KVStore.update(Map): g = sum / sumCnt, updater by key (exact, prefix, "default"), then clear (:240-277)
-        char key[32];
-        snprintf(key, sizeof key, "fc%d.weights", l);
-        ps_updater_t u;
-        PSCHK(store_resolve_updater(s, key, &u));
-        DenseUpdArgs d;
-        memset(&d, 0, sizeof d);
-        d.nlayers = 1; d.B = 1; d.apply = 1; d.flat_grad = p.pending; d.flat_div = (float)p.pending_cnt;
-        d.upd = make_upd_params(u);
-        DenseLayer &L = d.L[0];
-        L.W = p.W; L.Wt = p.Wt; L.Wp = p.Wp; L.S1 = p.S1; L.S2 = p.S2; L.K = p.K; L.N = p.N; L.ldw = p.ldw; L.ldwt = p.Kpad;
-        L.elem_begin = 0; L.elem_end = (int64_t)(p.K + 1) * p.N;
-        PSCHK(launch_dense_update(d, s->stream));
-        p.pending_cnt = 0;
-        ++done;
+        PSCHK(store_apply_pending(s, s->fc[l], "fc", l, &one));
+        done += one;
+    }
+    for (int l = 0; layer < 0 && l < (int)s->ln.size(); ++l) {
+        PSCHK(store_apply_pending(s, s->ln[l], "ln", l, &one));
+        done += one;
     }
     if (layer >= 0 && !done) return ps_set_err(PS_MISSING, "fc%d has no pending gradient", layer);
     if (done) s->global_step++;

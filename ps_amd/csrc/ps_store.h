@@ -57,6 +57,7 @@ struct ps_store {
     EmbTables emb;
     WideTable wide;
     std::vector<FcParams> fc;
+    std::vector<FcParams> ln;          // layer normalisations: K = 1, W' row 0 = "ln<i>.weights" (gamma), row 1 = "ln<i>.bias" (beta)
     std::map<std::string, ps_updater_t> updaters;
     int64_t global_step = 0;
     int64_t bytes = 0;
@@ -85,12 +86,25 @@ struct ps_store {
         uint32_t *keys = nullptr, *ents = nullptr, *ent_bag = nullptr, *seg_start = nullptr, *seg_id = nullptr, *nseg = nullptr, *uniq_row = nullptr;
         float *partials = nullptr, *partials2 = nullptr, *grads = nullptr;
     } ops;
+    // workspace of the residual tower's operators (ps_tower.hip), grow-only; a block that a recorded graph may still point to is kept
+    // until the store goes
+    struct TowerWs {
+        char *p = nullptr; size_t cap = 0; bool recorded = false;
+        std::vector<char *> retired;
+    } tower;
 };
 
 int store_dev_alloc(ps_store *s, void **p, size_t bytes, bool zero);
-// "emF<f>.<id>.0" | "wide.weights.<id>.0" | "wide.bias" | "fc<i>.weights" | "fc<i>.bias"
-struct ParsedKey { int kind; int idx; int64_t id; };  // kind 0 emb, 1 wide w, 2 wide bias, 3 fc w, 4 fc b
+// "emF<f>.<id>.0" | "wide.weights.<id>.0" | "wide.bias" | "fc<i>.weights" | "fc<i>.bias" | "ln<i>.weights" | "ln<i>.bias"
+struct ParsedKey { int kind; int idx; int64_t id; };  // kind 0 emb, 1 wide w, 2 wide bias, 3 fc w, 4 fc b, 5 ln w, 6 ln b
 bool store_parse_key(const char *key, ParsedKey *k);
+// the dense tensor a parsed key of kind >= 3 names (NULL: not held) and whether it is the tensor's bias row
+FcParams *store_dense(ps_store *s, const ParsedKey &k);
+static inline bool key_is_bias(const ParsedKey &k) { return k.kind == 4 || k.kind == 6; }
+static inline bool key_is_ln(const ParsedKey &k) { return k.kind >= 5; }
+// KVStore.update of a dense tensor's pending gradient (ps_layer_ops.hip); false: it has none
+int store_apply_pending(ps_store *s, FcParams &p, const char *stem, int layer, bool *done);
+#define PS_LN_MAX 64
 // PServer.push (+ psUpdate) of a list of (owner-local row, gradient) pairs; bump_step: globalStep.incrementAndGet()
 int shard_apply_push(ps_store *s, const uint32_t *rows_dev, const float *grads_dev, int64_t n, const int64_t *peer_counts,
                      int npeers, int is_async, bool bump_step);

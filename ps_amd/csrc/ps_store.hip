@@ -293,7 +293,10 @@ extern "C" int ps_store_destroy(ps_store_t *s) {
     fr(s->emb.W); fr(s->emb.state); fr(s->emb.row_base_dev);
     fr(s->emb.owner_dev); fr(s->emb.local_dev); fr(s->emb.grow_base_dev);
     fr(s->wide.W); fr(s->wide.state); fr(s->wide.touched); fr(s->wide.bias); fr(s->wide.bias_state);
-    for (auto &f : s->fc) { fr(f.W); fr(f.Wt); fr(f.Wp); fr(f.S1); fr(f.S2); fr(f.pending); }
+    for (auto *v : {&s->fc, &s->ln})
+        for (auto &f : *v) { fr(f.W); fr(f.Wt); fr(f.Wp); fr(f.S1); fr(f.S2); fr(f.pending); }
+    fr(s->tower.p);
+    for (char *p : s->tower.retired) fr(p);
     {
         ps_store::OpScratch &o = s->ops;
         sort_ws_free(o.ws);
@@ -614,6 +617,37 @@ extern "C" int ps_store_create_fc(ps_store_t *s, int layer, int in_dims, int out
     return PS_OK;
 }
 
+extern "C" int ps_store_create_ln(ps_store_t *s, int layer, int dims) {
+    if (!s || layer < 0 || layer >= PS_LN_MAX || dims <= 0 || dims > (1 << 20)) return ps_set_err(PS_E_BAD_ARG, "bad normalisation layer");
+    PSCHK(store_enter(s));
+    if (layer < (int)s->ln.size() && s->ln[layer].present) {
+        if (s->ln[layer].N != dims) return ps_set_err(PS_E_STATE, "ln%d exists with another width", layer);
+        return PS_OK;
+    }
+    try {
+        if ((int)s->ln.size() <= layer) s->ln.resize(layer + 1);
+    } catch (...) { return ps_set_err(PS_E_HIP, "out of host memory"); }
+    FcParams f;
+    f.K = 1; f.N = dims; f.Kpad = 2;
+    f.ldw = (int)round_up(dims, 16);
+    const size_t wn = (size_t)f.Kpad * f.ldw;
+    // (a failure half-way leaves the layer absent and frees what it had)
+    auto drop = [&](int rc) { RtGuard g; for (float *p : {f.W, f.Wt, f.S1, f.S2, f.pending}) if (p) (void)hipFree(p); return rc; };
+    int rc = PS_OK;
+    for (float **p : {&f.W, &f.S1, &f.S2})
+        if (rc == PS_OK) rc = store_dev_alloc(s, (void **)p, sizeof(float) * wn, true);
+    if (rc == PS_OK) rc = store_dev_alloc(s, (void **)&f.Wt, sizeof(float) * (size_t)f.Kpad * f.N, true);
+    if (rc == PS_OK) rc = store_dev_alloc(s, (void **)&f.pending, sizeof(float) * 2 * (size_t)f.N, true);
+    if (rc == PS_OK) rc = launch_fill(f.W, dims, 1.f, s->stream);
+    if (rc == PS_OK) rc = launch_transpose_w(f.W, f.Wt, f.Kpad, f.ldw, f.N, s->stream);
+    if (rc != PS_OK) return drop(rc);
+    const hipError_t e = hipStreamSynchronize(s->stream);
+    if (e != hipSuccess) return drop(ps_set_err(PS_E_HIP, "ln%d: %s", layer, hipGetErrorString(e)));
+    f.present = true;
+    s->ln[layer] = f;
+    return PS_OK;
+}
+
 int64_t store_local_row(const ps_store *s, int field, int64_t id) {
     const EmbTables &e = s->emb;
     if (field < 0 || field >= e.F || id < 0 || id >= e.rows[field]) return -1;
@@ -693,7 +727,7 @@ extern "C" int ps_store_put_wide(ps_store_t *s, const int64_t *ids, int64_t n, i
 }
 
 // ---- string keys ------------------------------------------------------------
-// "emF<f>.<id>.0" | "wide.weights.<id>.0" | "wide.bias" | "fc<i>.weights" | "fc<i>.bias"
+// "emF<f>.<id>.0" | "wide.weights.<id>.0" | "wide.bias" | "fc<i>.weights" | "fc<i>.bias" | "ln<i>.weights" | "ln<i>.bias"
 static bool parse_float_id(const char *p, int64_t *id) {
     char *e = nullptr;
     const double v = strtod(p, &e);                  // "28305.0" (also accepts "2.8305E4")
@@ -720,13 +754,28 @@ static bool parse_key(const char *key, ParsedKey *k) {
         if (strcmp(e, ".weights") == 0) { k->kind = 3; return true; }
         if (strcmp(e, ".bias") == 0) { k->kind = 4; return true; }
     }
+    if (strncmp(key, "ln", 2) == 0) {
+        char *e = nullptr;
+        const long i = strtol(key + 2, &e, 10);
+        if (e == key + 2 || i < 0 || i >= PS_LN_MAX) return false;
+        k->idx = (int)i; k->id = 0;
+        if (strcmp(e, ".weights") == 0) { k->kind = 5; return true; }
+        if (strcmp(e, ".bias") == 0) { k->kind = 6; return true; }
+    }
     return false;
 }
 bool store_parse_key(const char *key, ParsedKey *k) { return parse_key(key, k); }
 
-static int fc_io(ps_store *s, int layer, int bias, float *host, int cap, int *len, int to_dev) {
-    if (layer < 0 || layer >= (int)s->fc.size() || !s->fc[layer].present) return ps_set_err(PS_MISSING, "fc%d absent", layer);
-    FcParams &f = s->fc[layer];
+FcParams *store_dense(ps_store *s, const ParsedKey &k) {
+    std::vector<FcParams> &v = key_is_ln(k) ? s->ln : s->fc;
+    return k.idx >= 0 && k.idx < (int)v.size() && v[k.idx].present ? &v[k.idx] : nullptr;
+}
+
+static int dense_io(ps_store *s, const char *key, const ParsedKey &pk, float *host, int cap, int *len, int to_dev) {
+    FcParams *fp = store_dense(s, pk);
+    if (!fp) return ps_set_err(PS_MISSING, "%s absent", key);
+    FcParams &f = *fp;
+    const bool bias = key_is_bias(pk);
     const int n = bias ? f.N : f.K * f.N;
     if (len) *len = n;
     if (cap < n) return ps_set_err(PS_E_BAD_ARG, "buffer too small: %d < %d", cap, n);
@@ -741,12 +790,7 @@ static int fc_io(ps_store *s, int layer, int bias, float *host, int cap, int *le
     }
     HIPCHK(hipMemcpy2DAsync(src, sizeof(float) * f.ldw, host, sizeof(float) * f.N, sizeof(float) * f.N, krows,
                             hipMemcpyHostToDevice, s->stream));
-    // keep the transposed copy in step: Wt[n][k]
-    std::vector<float> t((size_t)f.N * krows);
-    for (int k = 0; k < krows; ++k)
-        for (int n2 = 0; n2 < f.N; ++n2) t[(size_t)n2 * krows + k] = host[(size_t)k * f.N + n2];
-    HIPCHK(hipMemcpy2DAsync(f.Wt + (bias ? f.K : 0), sizeof(float) * f.Kpad, t.data(), sizeof(float) * krows,
-                            sizeof(float) * krows, f.N, hipMemcpyHostToDevice, s->stream));
+    PSCHK(launch_transpose_w(f.W, f.Wt, f.Kpad, f.ldw, f.N, s->stream));      // keep the transposed copy in step
     PSCHK(launch_pack_w(f.Wt, f.Wp, f.N, f.Kpad, s->stream));
     HIPCHK(hipStreamSynchronize(s->stream));
     return PS_OK;
@@ -774,8 +818,7 @@ extern "C" int ps_store_get(ps_store_t *s, const char *key, float *out, int cap,
         HIPCHK(hipMemcpyAsync(out, s->wide.bias, sizeof(float), hipMemcpyDeviceToHost, s->stream));
         HIPCHK(hipStreamSynchronize(s->stream));
         return PS_OK;
-    case 3: return fc_io(s, k.idx, 0, out, cap, len, 0);
-    default: return fc_io(s, k.idx, 1, out, cap, len, 0);
+    default: return dense_io(s, key, k, out, cap, len, 0);
     }
 }
 
@@ -798,7 +841,6 @@ extern "C" int ps_store_put(ps_store_t *s, const char *key, const float *val, in
         HIPCHK(hipMemcpyAsync(s->wide.bias, val, sizeof(float), hipMemcpyHostToDevice, s->stream));
         HIPCHK(hipStreamSynchronize(s->stream));
         return PS_OK;
-    case 3: return fc_io(s, k.idx, 0, const_cast<float *>(val), n, &len, 1);
-    default: return fc_io(s, k.idx, 1, const_cast<float *>(val), n, &len, 1);
+    default: return dense_io(s, key, k, const_cast<float *>(val), n, &len, 1);
     }
 }

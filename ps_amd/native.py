@@ -17,7 +17,8 @@ PS_UPD_ADAM, PS_UPD_FTRL, PS_UPD_SIMPLE = 0, 1, 2
 PS_ROUTE_ID_MOD, PS_ROUTE_JAVA_STRING = 0, 1
 PS_MODEL_DNN, PS_MODEL_WIDEDEEP = 0, 1
 PS_GRAD_COMPAT, PS_GRAD_INTENDED = 0, 1
-PS_ACT_NONE, PS_ACT_RELU, PS_ACT_SIGMOID = 0, 1, 2
+PS_ACT_NONE, PS_ACT_RELU, PS_ACT_SIGMOID, PS_ACT_GELU, PS_ACT_SILU = 0, 1, 2, 3, 4
+PS_T_F32, PS_T_BF16, PS_T_F16 = 0, 1, 2
 PS_SUM_AUTO, PS_SUM_SEQUENTIAL, PS_SUM_CHUNKED = 0, 1, 2
 
 
@@ -122,6 +123,13 @@ SIGNATURES = {
     "ps_fc_backward": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _i, _vp, _i]),
     "ps_fc_pending_grad": (_i, [_vp, _i, _i, _pf, _i, _pi]),
     "ps_dense_update": (_i, [_vp, _i]),
+    "ps_store_create_ln": (_i, [_vp, _i, _i]),
+    "ps_ln_forward": (_i, [_vp, _i, _i, _vp, _i64, _i, _f, _vp, _i64, _vp]),
+    "ps_ln_backward": (_i, [_vp, _i, _i, _vp, _i64, _vp, _vp, _i64, _i, _vp, _i64, _vp, _i64, _vp]),
+    "ps_ln_pending_grad": (_i, [_vp, _i, _i, _pf, _i, _pi]),
+    "ps_ln_update": (_i, [_vp, _i]),
+    "ps_fc_res_forward": (_i, [_vp, _i, _i, _i, _vp, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64]),
+    "ps_fc_res_backward": (_i, [_vp, _i, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _i64, _vp, _i64, _vp]),
     "ps_emb_backward_update": (_i, [_vp, _vp, _vp, _i64, _i, _i, _vp, _i, _vp, _i, _i, _i, _i]),
     "ps_emb_last_grads": (_i, [_vp, _pi64, _pf, _i64, _pi64]),
     "ps_store_set_stream": (_i, [_vp, _vp]),
