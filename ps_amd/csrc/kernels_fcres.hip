@@ -31,16 +31,41 @@ template <> struct Mma<float> {        // a fragment holds 4 steps of 2: the lan
     }
 };
 
-__device__ __forceinline__ float act_apply(float z, int act) {
-    if (act == PS_ACT_RELU) return z < 0.f ? 0.f : z;      // (a NaN stays one)
-    if (act == PS_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    if (act == PS_ACT_SILU) return z / (1.f + expf(-z));
-    return z;
+// The normal law's tail Q(|z|) = erfc(|z| / sqrt 2) / 2 and density: Abramowitz & Stegun 7.1.26 (|error of erfc| < 1.5e-7: about the
+// rounding of 1 + erf in f32), whose e^(-z^2 / 2) the slope needs anyway.  About 20 instruction slots with one reciprocal and one
+// exponential, a third of the library's erff -- in the epilogue of a product nothing hides them.
+__device__ __forceinline__ float normal_tail(float z, float &e) {
+    const float x = fabsf(z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, x, 1.f));
+    e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);                       // e^(-z^2 / 2)
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    return 0.5f * p * t * e;
+}
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
+template <int NV> __device__ __forceinline__ void act_apply(float (&v)[NV], int act) {
+    float e;
+    if (act == PS_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];        // (a NaN stays one)
+    } else if (act == PS_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = fmaf(-fabsf(v[j]), normal_tail(v[j], e), fmaxf(v[j], 0.f));      // z Phi(z) = max(z, 0) - |z| Q(|z|)
+    } else if (act == PS_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] *= logistic(v[j]);
+    }
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
-    if (act == PS_ACT_GELU) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-    const float p = 1.f / (1.f + expf(-z));
-    return p * (1.f + z * (1.f - p));
+    if (act == PS_ACT_GELU) {
+        float e;
+        const float q = normal_tail(z, e);
+        return fmaf(z * 0.39894228f, e, z < 0.f ? q : 1.f - q);
+    }
+    const float p = logistic(z);
+    return p * fmaf(z, 1.f - p, 1.f);
 }
 
 // workgroup -> tile so that an XCD (workgroup id mod 8) owns a contiguous range of tiles: its L2 then serves the tiles' shared rows
@@ -157,17 +182,207 @@ __global__ __launch_bounds__(256) void k_fc_nt(FcNtArgs a, int tiles_n) {
 #pragma unroll
             for (int q = 0; q < GR; ++q) {
                 const int n = n0 + wn + i * TILE + q * 8 + lg * 4;
+                float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (n + e >= a.N) continue;
-                    float v = acc[i][j][q * 4 + e];
-                    if (a.bias) v += a.bias[n + e];
-                    if (a.Z) zr[n + e] = (T)v;
-                    v = act_apply(v, a.act);
-                    if (a.R) v += (float)rr[n + e];
-                    y[n + e] = (T)v;
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e] + (a.bias && n + e < a.N ? a.bias[n + e] : 0.f);
+                if (a.Z) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < a.N) zr[n + e] = (T)v[e];
                 }
+                act_apply(v, a.act);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.N) y[n + e] = (T)(a.R ? v[e] + (float)rr[n + e] : v[e]);
             }
+    }
+}
+
+// The weights of a product in the activations' type, laid out for k_fc_nt_big: rows padded with zeros to a multiple of BK and of BN
+template <typename T> __global__ __launch_bounds__(256) void k_cast_w(const float *__restrict__ W, int ldw, int N, int K, T *__restrict__ out, int Kp, int Np) {
+    const int per = Kp / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)per * Np) return;
+    const int n = (int)(i / per), c = (int)(i % per) * 8;
+    Chunk<T> o;
+    o.zero();
+    if (n < N && c < K) load_w<T>(o, W + (size_t)n * ldw, c, K);
+    *reinterpret_cast<u32x4 *>(out + (size_t)n * Kp + c) = o.u;
+}
+
+constexpr int BIG_M = 256, BIG_N = 256, BIG_K = 64, BIG_GROUP = 8;
+typedef __attribute__((address_space(3))) void lds_void;
+#define PS_WAIT_LOADS(n) asm volatile("s_waitcnt vmcnt(" #n ") lgkmcnt(0)" ::: "memory")
+
+// 16-bit operands, a 256 x 256 tile per workgroup of 8 waves (2 x 4, 128 x 64 each), one workgroup a CU: the tile that asks least of L2
+// and of LDS per product.  Both operands go straight from memory into LDS (no registers, no conversion: the weights were cast once).
+// LDS holds two steps of 64 along the sum, each in four quarters (x's rows by their wave's upper and lower half, the weights' by their
+// wave's half too), and a step is four phases of 16 matrix instructions, each over a quarter of the wave's tile:
+//      phase 0: read x0, w0 -- x0 w0      1: read w1 -- x0 w1      2: read x1 -- x1 w1      3: x1 w0
+// A quarter is free once its phase has read it, and is asked for again -- two steps ahead -- in the phase after that: one quarter (two
+// loads a lane) per phase, five quarters in flight, so what a phase reads was asked for five phases ago (vmcnt(10)).
+// The two waves of a SIMD work in turn: one reads and asks for memory while the other multiplies; a barrier ends every half phase and
+// the second four waves run one half phase behind.
+// LDS rows are 128 bytes, 16-byte pieces exchanged by a row key so that 8 neighbouring lanes of a fragment read touch different banks;
+// the exchange is made in the loads' addresses, LDS itself is written in lane order.  A wave's weight rows are dealt to its four
+// fragments in groups of 4, so that a lane ends with 16 neighbouring columns of a row of y: whole 128-byte lines per row and wave.
+// Rows of x behind the last read as zeros through the buffer's bound; a last step that K does not fill goes through registers, where
+// its tail is cut off.
+template <typename T>
+__global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, int Kp, int tiles_m, int tiles_n) {
+    typedef Mma<T> X;
+    typedef typename X::frag frag;
+    constexpr int Q = 128 * 8;                   // pieces of a quarter
+    // (one array for everything: with several the compiler tells their loads apart and waits for all of them before a read of any)
+    __shared__ u32x4 lds[2][4 * Q];              // [step][x0 | w0 | w1 | x1]
+    int tm, tn;
+    {   // an XCD's tiles in groups of BIG_GROUP rows of tiles: what runs on it at one time shares rows of x and of the weights in its L2
+        const int tile = xcd_tile(blockIdx.x, gridDim.x), per = BIG_GROUP * tiles_n, g = tile / per, left = tiles_m - g * BIG_GROUP;
+        const int gm = left < BIG_GROUP ? left : BIG_GROUP;
+        tm = g * BIG_GROUP + (tile % per) % gm; tn = (tile % per) / gm;
+    }
+    const int64_t m0 = (int64_t)tm * BIG_M;
+    const int n0 = tn * BIG_N;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+    const T *A0 = (const T *)a.A + m0 * a.lda;
+    const int64_t rows = a.M - m0 < BIG_M ? a.M - m0 : BIG_M;
+    auto rsA = __builtin_amdgcn_make_buffer_rsrc((void *)A0, 0, (int)(((rows - 1) * a.lda + a.K) * 2), 0x00020000);
+    auto rsB = __builtin_amdgcn_make_buffer_rsrc((void *)(Wc + (size_t)n0 * Kp), 0, BIG_N * Kp * 2, 0x00020000);
+    // row q of a quarter: x's row (q / 64) * 128 + half * 64 + q % 64, the weights' row (q / 32) * 64 + (q / 8 % 4) * 16 + half * 8 + q % 8
+    const int q = tid >> 3, pc = tid & 7, ca = (pc ^ (q & 7)) * 16, cb = (pc ^ ((q & 3) | ((q >> 1) & 4))) * 16;
+    int va[4];                                   // [half * 2 + i]: in the lane's offset, which the bound is checked with
+#pragma unroll
+    for (int i = 0; i < 4; ++i) va[i] = (int)((q + (i & 1) * 128 + (i >> 1) * 64) * a.lda * 2) + ca;
+    const int vb = ((q >> 5) * 64 + ((q >> 3) & 3) * 16 + (q & 7)) * Kp * 2 + cb, sb = Kp * 2;
+    auto ask_x = [&](int t, int half) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_void *)&lds[t & 1][(half ? 3 : 0) * Q + i * 512 + wave * 64], 16, va[half * 2 + i], t * 128, 0, 0);
+    };
+    auto ask_w = [&](int t, int half) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_void *)&lds[t & 1][(1 + half) * Q + i * 512 + wave * 64], 16, vb, t * 128 + (i * 128 + half * 8) * sb, 0, 0);
+    };
+    f32x4 acc[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int lr = lane & 15, lg = lane >> 4;
+    frag fx[2][4], fw[2][4];                     // [step of 32][fragment]
+    int ox[2], ow[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        ox[k] = (wm * 64 + lr) * 8 + ((k * 4 + lg) ^ (lr & 7));
+        const int r = wn * 32 + (lr >> 2) * 8 + (lr & 3);
+        ow[k] = r * 8 + ((k * 4 + lg) ^ ((r & 3) | ((r >> 1) & 4)));
+    }
+    auto read_x = [&](int t, int half) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fx[k][j] = *reinterpret_cast<const frag *>(&lds[t & 1][(half ? 3 : 0) * Q + ox[k] + j * 128]);
+    };
+    auto read_w = [&](int t, int half) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) fw[k][half * 2 + i] = *reinterpret_cast<const frag *>(&lds[t & 1][(1 + half) * Q + ow[k] + i * 32]);
+    };
+    auto multiply = [&](int hx, int hw) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) acc[hw * 2 + i][hx * 4 + j] = X::mma(fw[k][hw * 2 + i], fx[k][j], acc[hw * 2 + i][hx * 4 + j]);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto turn = [&]() { __builtin_amdgcn_sched_barrier(0); __builtin_amdgcn_s_barrier(); __builtin_amdgcn_sched_barrier(0); };
+    const int steps = a.K / BIG_K;
+    if (steps > 0) { ask_x(0, 0); ask_w(0, 0); ask_w(0, 1); ask_x(0, 1); }
+    if (steps > 1) {
+        ask_x(1, 0); ask_w(1, 0); ask_w(1, 1);
+        PS_WAIT_LOADS(10);
+    } else {
+        PS_WAIT_LOADS(0);
+    }
+    turn();
+    if (wm) turn();                              // the second four waves: half a phase behind from here on
+    int t = 0;
+    for (; t < steps - 2; ++t) {
+        read_x(t, 0); read_w(t, 0); ask_x(t + 1, 1);
+        PS_WAIT_LOADS(10); turn(); multiply(0, 0); turn();
+        read_w(t, 1); ask_x(t + 2, 0);
+        PS_WAIT_LOADS(10); turn(); multiply(0, 1); turn();
+        read_x(t, 1); ask_w(t + 2, 0);
+        PS_WAIT_LOADS(10); turn(); multiply(1, 1); turn();
+        ask_w(t + 2, 1);
+        PS_WAIT_LOADS(10); turn(); multiply(1, 0); turn();
+    }
+    for (; t < steps; ++t) {                     // the last two: nothing but x1 is left to ask for
+        read_x(t, 0); read_w(t, 0);
+        if (t + 1 < steps) ask_x(t + 1, 1);
+        PS_WAIT_LOADS(0); turn(); multiply(0, 0); turn();
+        read_w(t, 1);
+        PS_WAIT_LOADS(0); turn(); multiply(0, 1); turn();
+        read_x(t, 1);
+        PS_WAIT_LOADS(0); turn(); multiply(1, 1); turn();
+        turn(); multiply(1, 0); turn();
+    }
+    if (!wm) turn();
+    if (a.K % BIG_K) {                           // every wave has read all there was; all eight in step from here on
+        ask_w(steps, 0); ask_w(steps, 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = q + (i & 1) * 128 + (i >> 1) * 64;
+            Chunk<T> c;
+            c.zero();
+            if (r < rows) c.load(A0 + r * a.lda, steps * BIG_K + ca / 2, a.K);
+            lds[steps & 1][(i >> 1 ? 3 : 0) * Q + (i & 1) * 512 + tid] = c.u;
+        }
+        PS_WAIT_LOADS(0);
+        turn();
+        read_x(steps, 0); read_w(steps, 0); read_w(steps, 1);
+        multiply(0, 0); multiply(0, 1);
+        read_x(steps, 1);
+        multiply(1, 1); multiply(1, 0);
+    }
+    const int n = n0 + wn * 64 + lg * 16;
+    if (n >= a.N) return;
+    float bias[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) bias[e] = a.bias ? a.bias[n + e] : 0.f;      // (the bias row is padded to a multiple of 16)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int64_t m = m0 + wm * 128 + j * 16 + lr;
+        if (m >= a.M) continue;
+        float v[16];
+        Chunk<T> o;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = acc[e >> 2][j][e & 3] + bias[e];
+        if (a.Z) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.e[e] = (T)v[h * 8 + e];
+                o.store((T *)a.Z + m * a.ldz, n + h * 8, a.N);
+            }
+        }
+        act_apply(v, a.act);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (a.R) {
+                o.load((const T *)a.R + m * a.ldr, n + h * 8, a.N);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[h * 8 + e] += (float)o.e[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o.e[e] = (T)v[h * 8 + e];
+            o.store((T *)a.Y + m * a.ldy, n + h * 8, a.N);
+        }
     }
 }
 
@@ -321,6 +536,20 @@ template <typename T, int BM, int BN> int nt_go(const FcNtArgs &a, hipStream_t s
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
+// may the product take k_fc_nt_big?  Its loads want 16-byte pieces, its offsets 31 bits, and its tiles at least one for each CU
+bool big_fits(int type, const FcNtArgs &a) {
+    if (type == PS_T_F32 || (uintptr_t)a.A % 16 || a.lda % 8 || a.lda > (1 << 21) || a.K > (1 << 21)) return false;
+    return (int64_t)cdiv(a.M, BIG_M) * cdiv(a.N, BIG_N) >= 128;
+}
+template <typename T> int nt_big(const FcNtArgs &a, void *ws, hipStream_t st) {
+    const int Kp = (int)round_up(a.K, BIG_K), Np = (int)round_up(a.N, BIG_N), tiles_n = Np / BIG_N;
+    const int64_t pieces = (int64_t)Kp / 8 * Np, blocks = (int64_t)tiles_n * cdiv(a.M, BIG_M);
+    PSCHK(grid_ok(2 * blocks));
+    hipLaunchKernelGGL((k_cast_w<T>), dim3((unsigned)cdiv(pieces, 256)), dim3(256), 0, st, a.W, a.ldw, a.N, a.K, (T *)ws, Kp, Np);
+    hipLaunchKernelGGL((k_fc_nt_big<T>), dim3((unsigned)blocks), dim3(512), 0, st, a, (const T *)ws, Kp, cdiv(a.M, BIG_M), tiles_n);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
+}
 template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
     if ((int64_t)cdiv(a.M, 128) * cdiv(a.N, 128) >= 256) return nt_go<T, 128, 128>(a, st);
     return nt_go<T, 64, 64>(a, st);
@@ -344,7 +573,11 @@ int ag_t(int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void
 
 }  // namespace
 
-int launch_fc_nt(int type, const FcNtArgs &a, hipStream_t st) {
+size_t fc_nt_workspace(int type, const FcNtArgs &a) {
+    return big_fits(type, a) ? (size_t)round_up(a.K, BIG_K) * (size_t)round_up(a.N, BIG_N) * 2 : 0;
+}
+int launch_fc_nt(int type, const FcNtArgs &a, void *ws, hipStream_t st) {
+    if (big_fits(type, a)) return type == PS_T_BF16 ? nt_big<__bf16>(a, ws, st) : nt_big<_Float16>(a, ws, st);
     return type == PS_T_F32 ? nt_t<float>(a, st) : type == PS_T_BF16 ? nt_t<__bf16>(a, st) : nt_t<_Float16>(a, st);
 }
 int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st) {

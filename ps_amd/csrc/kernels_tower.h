@@ -37,7 +37,8 @@ struct FcNtArgs {
     void *Y; int64_t ldy;
     int M, N, K, act;
 };
-int launch_fc_nt(int type, const FcNtArgs &a, hipStream_t st);
+size_t fc_nt_workspace(int type, const FcNtArgs &a);                        // bytes of ws that launch_fc_nt needs, 16-byte aligned
+int launch_fc_nt(int type, const FcNtArgs &a, void *ws, hipStream_t st);
 // dz = dy * act'(z), rounded to the type; rows of lddz elements
 int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st);
 // part[s][k][n] = sum over the s-th part of m of X[m][k] * D[m][n], k < K; row K: the sum of D[m][n]
@@ -79,7 +80,7 @@ template <typename T> struct Chunk {
             if (c + j < n) e[j] = row[c + j];
     }
     __device__ __forceinline__ void store(T *row, int c, int n) const {
-        if (c + N <= n) { *reinterpret_cast<unaligned_t *>(row + c) = u; return; }
+                if (c + N <= n) { *reinterpret_cast<unaligned_t *>(row + c) = u; return; }
 #pragma unroll
         for (int j = 0; j < N; ++j)
             if (c + j < n) row[c + j] = e[j];

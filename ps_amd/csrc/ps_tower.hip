@@ -206,7 +206,10 @@ extern "C" int ps_fc_res_forward(ps_store_t *s, int layer, int type, int act, co
     FcNtArgs a;
     a.A = x_dev; a.lda = ldx; a.W = p->Wt; a.ldw = p->Kpad; a.bias = p->W + (size_t)p->K * p->ldw; a.R = r_dev; a.ldr = r_dev ? ldr : 0;
     a.Z = z_dev; a.ldz = z_dev ? ldz : 0; a.Y = y_dev; a.ldy = ldy; a.M = B; a.N = p->N; a.K = p->K; a.act = act;
-    return launch_fc_nt(type, a, s->stream);
+    const size_t need = fc_nt_workspace(type, a);
+    char *ws = nullptr;
+    if (need) PSCHK(workspace(s, need, &ws));
+    return launch_fc_nt(type, a, ws, s->stream);
 }
 
 extern "C" int ps_fc_res_backward(ps_store_t *s, int layer, int type, int act, const void *x_dev, int64_t ldx, const void *z_dev, int64_t ldz,
@@ -233,26 +236,23 @@ extern "C" int ps_fc_res_backward(ps_store_t *s, int layer, int type, int act, c
     float *dst;
     int accum;
     PSCHK(grad_target(s, *p, grad_dev, &dst, &accum));
-    // workspace: [slabs of dW | db][dz]
+    // workspace: [slabs of dW | db][dz][what the product for dx needs]
     const int nsplit = fc_tn_splits(type, B, K, N);
     const int64_t slab = (int64_t)(K + 1) * N, lddz = round_up(N, 8);
-    const size_t slabs = (size_t)round_up((int64_t)sizeof(float) * slab * nsplit, 256);
+    const size_t slabs = (size_t)round_up((int64_t)sizeof(float) * slab * nsplit, 256), dzs = z_dev ? (size_t)round_up(es * lddz * B, 256) : 0;
+    FcNtArgs a;
+    a.A = dy_dev; a.lda = lddy; a.W = p->W; a.ldw = p->ldw; a.bias = nullptr; a.R = skip_dev; a.ldr = skip_dev ? ldskip : 0; a.Z = nullptr; a.ldz = 0;
+    a.Y = dx_dev; a.ldy = lddx; a.M = B; a.N = K; a.K = N; a.act = PS_ACT_NONE;
+    if (z_dev) { a.A = nullptr; a.lda = lddz; }             // (dz: 256-byte aligned in the workspace)
     char *ws;
-    PSCHK(workspace(s, slabs + (z_dev ? (size_t)es * lddz * B : 0), &ws));
-    const void *d = dy_dev;
-    int64_t ldd = lddy;
+    PSCHK(workspace(s, slabs + dzs + (dx_dev ? fc_nt_workspace(type, a) : 0), &ws));
     if (z_dev) {
+        a.A = ws + slabs;
         PSCHK(launch_act_grad(type, act, dy_dev, lddy, z_dev, ldz, ws + slabs, lddz, B, N, st));
-        d = ws + slabs; ldd = lddz;
     }
-    if (dx_dev) {
-        FcNtArgs a;
-        a.A = d; a.lda = ldd; a.W = p->W; a.ldw = p->ldw; a.bias = nullptr; a.R = skip_dev; a.ldr = skip_dev ? ldskip : 0; a.Z = nullptr; a.ldz = 0;
-        a.Y = dx_dev; a.ldy = lddx; a.M = B; a.N = K; a.K = N; a.act = PS_ACT_NONE;
-        PSCHK(launch_fc_nt(type, a, st));
-    }
+    if (dx_dev) PSCHK(launch_fc_nt(type, a, ws + slabs + dzs, st));
     FcTnArgs t;
-    t.X = x_dev; t.ldx = ldx; t.D = d; t.ldd = ldd; t.part = (float *)ws; t.M = B; t.K = K; t.N = N; t.nsplit = nsplit;
+    t.X = x_dev; t.ldx = ldx; t.D = a.A; t.ldd = a.lda; t.part = (float *)ws; t.M = B; t.K = K; t.N = N; t.nsplit = nsplit;
     PSCHK(launch_fc_tn(type, t, st));
     PSCHK(launch_grad_reduce(t.part, nsplit, slab, slab, B, dst, accum, st));
     if (!grad_dev) p->pending_cnt++;
