@@ -210,71 +210,83 @@ template <typename T> __global__ __launch_bounds__(256) void k_cast_w(const floa
     *reinterpret_cast<u32x4 *>(out + (size_t)n * Kp + c) = o.u;
 }
 
-constexpr int BIG_M = 256, BIG_N = 256, BIG_K = 64, BIG_GROUP = 8;
+constexpr int BIG_M = 256, BIG_K = 64, BIG_GROUP = 8;
 typedef __attribute__((address_space(3))) void lds_void;
-#define PS_WAIT_LOADS(n) asm volatile("s_waitcnt vmcnt(" #n ") lgkmcnt(0)" ::: "memory")
+// all but the last n loads have landed and every LDS read has returned (the builtin, which the compiler's own wait counting sees: behind
+// waits written in assembly it took an epilogue's loads for still pending and waited for everything inside the product's loop)
+#define PS_WAIT_LOADS(n)                                                        \
+    do {                                                                        \
+        asm volatile("" ::: "memory");                                          \
+        __builtin_amdgcn_s_waitcnt(((n) & 15) | 0x70 | (((n) >> 4) << 14));     \
+        asm volatile("" ::: "memory");                                          \
+    } while (0)
 
-// 16-bit operands, a 256 x 256 tile per workgroup of 8 waves (2 x 4, 128 x 64 each), one workgroup a CU: the tile that asks least of L2
-// and of LDS per product.  Both operands go straight from memory into LDS (no registers, no conversion: the weights were cast once).
+// 16-bit operands, a 256 x BN tile per workgroup of 8 waves, one workgroup a CU.  BN = 256 (waves
+// 2 x 4, 128 x 64 each) asks least of L2 and of LDS per product; BN = 128 (waves 4 x 2, 64 x 64 each) is for outputs of so few tiles
+// that half the chip would idle.
+// Both operands go straight from memory into LDS (no registers, no conversion: the weights were cast once).
 // LDS holds two steps of 64 along the sum, each in four quarters (x's rows by their wave's upper and lower half, the weights' by their
-// wave's half too), and a step is four phases of 16 matrix instructions, each over a quarter of the wave's tile:
+// wave's half too), and a step is four phases, each over a quarter of the wave's tile (16 or 8 matrix instructions):
 //      phase 0: read x0, w0 -- x0 w0      1: read w1 -- x0 w1      2: read x1 -- x1 w1      3: x1 w0
-// A quarter is free once its phase has read it, and is asked for again -- two steps ahead -- in the phase after that: one quarter (two
-// loads a lane) per phase, five quarters in flight, so what a phase reads was asked for five phases ago (vmcnt(10)).
+// A quarter is free once its phase has read it, and is asked for again -- two steps ahead -- in the phase after that: one quarter per
+// phase, five quarters in flight; what a phase reads was asked for five phases ago (the waits count the loads since).
 // The two waves of a SIMD work in turn: one reads and asks for memory while the other multiplies; a barrier ends every half phase and
 // the second four waves run one half phase behind.
+// (A workgroup that walked several tiles, asking for the next one's first quarters before storing, lost: its load counts wait for its
+// stores, a new workgroup's do not -- 347 against 326 us for 32768 x 1024 -> 4096 with GELU.)
 // LDS rows are 128 bytes, 16-byte pieces exchanged by a row key so that 8 neighbouring lanes of a fragment read touch different banks;
 // the exchange is made in the loads' addresses, LDS itself is written in lane order.  A wave's weight rows are dealt to its four
-// fragments in groups of 4, so that a lane ends with 16 neighbouring columns of a row of y: whole 128-byte lines per row and wave.
+// fragments in groups of 4, so that a lane ends with 16 neighbouring columns of a row of y: whole 128-byte lines per row and wave (1-3 %
+// faster than 64 bytes of four lanes per store).
 // Rows of x behind the last read as zeros through the buffer's bound; a last step that K does not fill goes through registers, where
 // its tail is cut off.
-template <typename T>
+template <typename T, int BN>
 __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, int Kp, int tiles_m, int tiles_n) {
     typedef Mma<T> X;
     typedef typename X::frag frag;
-    constexpr int Q = 128 * 8;                   // pieces of a quarter
+    constexpr int WN = BN / 64, WM = 8 / WN, HX = BIG_M / WM / 2, FJ = HX / 16;      // waves along n and m; rows and fragments of half a wave's x
+    constexpr int QX = 128 * 8, QW = BN / 2 * 8, LX = 2, LW = QW / 512;              // pieces of a quarter, loads of a lane for it
+    constexpr int OX[2] = {0, QX + 2 * QW}, OW[2] = {QX, QX + QW};
     // (one array for everything: with several the compiler tells their loads apart and waits for all of them before a read of any)
-    __shared__ u32x4 lds[2][4 * Q];              // [step][x0 | w0 | w1 | x1]
-    int tm, tn;
-    {   // an XCD's tiles in groups of BIG_GROUP rows of tiles: what runs on it at one time shares rows of x and of the weights in its L2
-        const int tile = xcd_tile(blockIdx.x, gridDim.x), per = BIG_GROUP * tiles_n, g = tile / per, left = tiles_m - g * BIG_GROUP;
-        const int gm = left < BIG_GROUP ? left : BIG_GROUP;
-        tm = g * BIG_GROUP + (tile % per) % gm; tn = (tile % per) / gm;
-    }
-    const int64_t m0 = (int64_t)tm * BIG_M;
-    const int n0 = tn * BIG_N;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+    __shared__ u32x4 lds[2][2 * QX + 2 * QW];    // [step][x0 | w0 | w1 | x1]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+    const bool second = wave >= 4;
+    const int sb = Kp * 2;
+    // row q of a quarter: x's row (q / HX) * 2 HX + half * HX + q % HX, the weights' row (q / 32) * 64 + (q / 8 % 4) * 16 + half * 8 + q % 8
+    const int q = tid >> 3, pc = tid & 7, ca = (pc ^ (q & 7)) * 16, cb = (pc ^ ((q & 3) | ((q >> 1) & 4))) * 16;
+    const int rx = (q / HX) * 2 * HX + q % HX;                                       // x's row of the lane's first piece; the second one's is 128 on
+    int va[2][2];                                                                    // in the lane's offset, which the bound is checked with
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) va[h][i] = (int)((rx + i * 128 + h * HX) * a.lda * 2) + ca;
+    const int vb = ((q >> 5) * 64 + ((q >> 3) & 3) * 16 + (q & 7)) * sb + cb;
+    // an XCD's tiles in groups of BIG_GROUP rows of tiles: what runs on it at one time shares rows of x and of the weights in its L2
+    const int tile = xcd_tile(blockIdx.x, gridDim.x), per = BIG_GROUP * tiles_n, g = tile / per, left = tiles_m - g * BIG_GROUP;
+    const int gm = left < BIG_GROUP ? left : BIG_GROUP;
+    const int64_t m0 = (int64_t)(g * BIG_GROUP + (tile % per) % gm) * BIG_M;
+    const int n0 = (tile % per) / gm * BN;
     const T *A0 = (const T *)a.A + m0 * a.lda;
     const int64_t rows = a.M - m0 < BIG_M ? a.M - m0 : BIG_M;
-    auto rsA = __builtin_amdgcn_make_buffer_rsrc((void *)A0, 0, (int)(((rows - 1) * a.lda + a.K) * 2), 0x00020000);
-    auto rsB = __builtin_amdgcn_make_buffer_rsrc((void *)(Wc + (size_t)n0 * Kp), 0, BIG_N * Kp * 2, 0x00020000);
-    // row q of a quarter: x's row (q / 64) * 128 + half * 64 + q % 64, the weights' row (q / 32) * 64 + (q / 8 % 4) * 16 + half * 8 + q % 8
-    const int q = tid >> 3, pc = tid & 7, ca = (pc ^ (q & 7)) * 16, cb = (pc ^ ((q & 3) | ((q >> 1) & 4))) * 16;
-    int va[4];                                   // [half * 2 + i]: in the lane's offset, which the bound is checked with
-#pragma unroll
-    for (int i = 0; i < 4; ++i) va[i] = (int)((q + (i & 1) * 128 + (i >> 1) * 64) * a.lda * 2) + ca;
-    const int vb = ((q >> 5) * 64 + ((q >> 3) & 3) * 16 + (q & 7)) * Kp * 2 + cb, sb = Kp * 2;
+    const auto rsA = __builtin_amdgcn_make_buffer_rsrc((void *)A0, 0, (int)(((rows - 1) * a.lda + a.K) * 2), 0x00020000);
+    const auto rsB = __builtin_amdgcn_make_buffer_rsrc((void *)(Wc + (size_t)n0 * Kp), 0, BN * sb, 0x00020000);
     auto ask_x = [&](int t, int half) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_void *)&lds[t & 1][(half ? 3 : 0) * Q + i * 512 + wave * 64], 16, va[half * 2 + i], t * 128, 0, 0);
+        for (int i = 0; i < LX; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_void *)&lds[t & 1][OX[half] + i * 512 + wave * 64], 16, va[half][i], t * 128, 0, 0);
     };
     auto ask_w = [&](int t, int half) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_void *)&lds[t & 1][(1 + half) * Q + i * 512 + wave * 64], 16, vb, t * 128 + (i * 128 + half * 8) * sb, 0, 0);
+        for (int i = 0; i < LW; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_void *)&lds[t & 1][OW[half] + i * 512 + wave * 64], 16, vb, t * 128 + (i * 128 + half * 8) * sb, 0, 0);
     };
-    f32x4 acc[4][8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[4][2 * FJ];
     const int lr = lane & 15, lg = lane >> 4;
-    frag fx[2][4], fw[2][4];                     // [step of 32][fragment]
+    frag fx[2][FJ], fw[2][4];                    // [step of 32][fragment]
     int ox[2], ow[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        ox[k] = (wm * 64 + lr) * 8 + ((k * 4 + lg) ^ (lr & 7));
+        ox[k] = (wm * HX + lr) * 8 + ((k * 4 + lg) ^ (lr & 7));
         const int r = wn * 32 + (lr >> 2) * 8 + (lr & 3);
         ow[k] = r * 8 + ((k * 4 + lg) ^ ((r & 3) | ((r >> 1) & 4)));
     }
@@ -282,22 +294,22 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) fx[k][j] = *reinterpret_cast<const frag *>(&lds[t & 1][(half ? 3 : 0) * Q + ox[k] + j * 128]);
+            for (int j = 0; j < FJ; ++j) fx[k][j] = *reinterpret_cast<const frag *>(&lds[t & 1][OX[half] + ox[k] + j * 128]);
     };
     auto read_w = [&](int t, int half) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) fw[k][half * 2 + i] = *reinterpret_cast<const frag *>(&lds[t & 1][(1 + half) * Q + ow[k] + i * 32]);
+            for (int i = 0; i < 2; ++i) fw[k][half * 2 + i] = *reinterpret_cast<const frag *>(&lds[t & 1][OW[half] + ow[k] + i * 32]);
     };
     auto multiply = [&](int hx, int hw) {
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < FJ; ++j)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) acc[hw * 2 + i][hx * 4 + j] = X::mma(fw[k][hw * 2 + i], fx[k][j], acc[hw * 2 + i][hx * 4 + j]);
+                for (int i = 0; i < 2; ++i) acc[hw * 2 + i][hx * FJ + j] = X::mma(fw[k][hw * 2 + i], fx[k][j], acc[hw * 2 + i][hx * FJ + j]);
         __builtin_amdgcn_s_setprio(0);
     };
     auto turn = [&]() { __builtin_amdgcn_sched_barrier(0); __builtin_amdgcn_s_barrier(); __builtin_amdgcn_sched_barrier(0); };
@@ -305,22 +317,26 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
     if (steps > 0) { ask_x(0, 0); ask_w(0, 0); ask_w(0, 1); ask_x(0, 1); }
     if (steps > 1) {
         ask_x(1, 0); ask_w(1, 0); ask_w(1, 1);
-        PS_WAIT_LOADS(10);
+        PS_WAIT_LOADS(2 * LX + 3 * LW);
     } else {
         PS_WAIT_LOADS(0);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2 * FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     turn();
-    if (wm) turn();                              // the second four waves: half a phase behind from here on
+    if (second) turn();                          // half a phase behind from here on
     int t = 0;
     for (; t < steps - 2; ++t) {
         read_x(t, 0); read_w(t, 0); ask_x(t + 1, 1);
-        PS_WAIT_LOADS(10); turn(); multiply(0, 0); turn();
+        PS_WAIT_LOADS(3 * LX + 2 * LW); turn(); multiply(0, 0); turn();
         read_w(t, 1); ask_x(t + 2, 0);
-        PS_WAIT_LOADS(10); turn(); multiply(0, 1); turn();
+        PS_WAIT_LOADS(3 * LX + 2 * LW); turn(); multiply(0, 1); turn();
         read_x(t, 1); ask_w(t + 2, 0);
-        PS_WAIT_LOADS(10); turn(); multiply(1, 1); turn();
+        PS_WAIT_LOADS(2 * LX + 3 * LW); turn(); multiply(1, 1); turn();
         ask_w(t + 2, 1);
-        PS_WAIT_LOADS(10); turn(); multiply(1, 0); turn();
+        PS_WAIT_LOADS(2 * LX + 3 * LW); turn(); multiply(1, 0); turn();
     }
     for (; t < steps; ++t) {                     // the last two: nothing but x1 is left to ask for
         read_x(t, 0); read_w(t, 0);
@@ -332,16 +348,16 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
         PS_WAIT_LOADS(0); turn(); multiply(1, 1); turn();
         turn(); multiply(1, 0); turn();
     }
-    if (!wm) turn();
+    if (!second) turn();
     if (a.K % BIG_K) {                           // every wave has read all there was; all eight in step from here on
         ask_w(steps, 0); ask_w(steps, 1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int64_t r = q + (i & 1) * 128 + (i >> 1) * 64;
+            const int64_t r = rx + (i & 1) * 128 + (i >> 1) * HX;
             Chunk<T> c;
             c.zero();
             if (r < rows) c.load(A0 + r * a.lda, steps * BIG_K + ca / 2, a.K);
-            lds[steps & 1][(i >> 1 ? 3 : 0) * Q + (i & 1) * 512 + tid] = c.u;
+            lds[steps & 1][OX[i >> 1] + (i & 1) * 512 + tid] = c.u;
         }
         PS_WAIT_LOADS(0);
         turn();
@@ -356,8 +372,8 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
 #pragma unroll
     for (int e = 0; e < 16; ++e) bias[e] = a.bias ? a.bias[n + e] : 0.f;      // (the bias row is padded to a multiple of 16)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int64_t m = m0 + wm * 128 + j * 16 + lr;
+    for (int j = 0; j < 2 * FJ; ++j) {
+        const int64_t m = m0 + wm * 2 * HX + j * 16 + lr;
         if (m >= a.M) continue;
         float v[16];
         Chunk<T> o;
@@ -536,17 +552,21 @@ template <typename T, int BM, int BN> int nt_go(const FcNtArgs &a, hipStream_t s
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
-// may the product take k_fc_nt_big?  Its loads want 16-byte pieces, its offsets 31 bits, and its tiles at least one for each CU
-bool big_fits(int type, const FcNtArgs &a) {
-    if (type == PS_T_F32 || (uintptr_t)a.A % 16 || a.lda % 8 || a.lda > (1 << 21) || a.K > (1 << 21)) return false;
-    return (int64_t)cdiv(a.M, BIG_M) * cdiv(a.N, BIG_N) >= 128;
+// Which tile of k_fc_nt_big a product takes, 0: none.  Its loads want 16-byte pieces and its offsets 31 bits; 128 columns cost 0.6 of
+// 256 (measured on full chips), so they win where they halve the rounds of the 256 CUs; below half a round the small tiles win.
+int big_tile(int type, const FcNtArgs &a) {
+    if (type == PS_T_F32 || (uintptr_t)a.A % 16 || a.lda % 8 || a.lda > (1 << 21) || a.K > (1 << 21)) return 0;
+    const int64_t tm = cdiv(a.M, BIG_M), t2 = tm * cdiv(a.N, 256), t1 = tm * cdiv(a.N, 128);
+    if (t1 < 128 || t1 >= (1 << 30)) return 0;
+    return 10 * cdiv(t2, 256) <= 6 * cdiv(t1, 256) ? 256 : 128;
 }
-template <typename T> int nt_big(const FcNtArgs &a, void *ws, hipStream_t st) {
-    const int Kp = (int)round_up(a.K, BIG_K), Np = (int)round_up(a.N, BIG_N), tiles_n = Np / BIG_N;
-    const int64_t pieces = (int64_t)Kp / 8 * Np, blocks = (int64_t)tiles_n * cdiv(a.M, BIG_M);
-    PSCHK(grid_ok(2 * blocks));
+template <typename T, int BN> int nt_big(const FcNtArgs &a, void *ws, hipStream_t st) {
+    const int Kp = (int)round_up(a.K, BIG_K), Np = (int)round_up(a.N, BN), tiles_n = Np / BN, tiles_m = cdiv(a.M, BIG_M);
+    const int64_t pieces = (int64_t)Kp / 8 * Np;
+    PSCHK(grid_ok(cdiv(pieces, 256)));
     hipLaunchKernelGGL((k_cast_w<T>), dim3((unsigned)cdiv(pieces, 256)), dim3(256), 0, st, a.W, a.ldw, a.N, a.K, (T *)ws, Kp, Np);
-    hipLaunchKernelGGL((k_fc_nt_big<T>), dim3((unsigned)blocks), dim3(512), 0, st, a, (const T *)ws, Kp, cdiv(a.M, BIG_M), tiles_n);
+    PSCHK(grid_ok(2ll * tiles_m * tiles_n));
+    hipLaunchKernelGGL((k_fc_nt_big<T, BN>), dim3((unsigned)(tiles_m * tiles_n)), dim3(512), 0, st, a, (const T *)ws, Kp, tiles_m, tiles_n);
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
@@ -574,10 +594,13 @@ int ag_t(int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void
 }  // namespace
 
 size_t fc_nt_workspace(int type, const FcNtArgs &a) {
-    return big_fits(type, a) ? (size_t)round_up(a.K, BIG_K) * (size_t)round_up(a.N, BIG_N) * 2 : 0;
+    const int bn = big_tile(type, a);
+    return bn ? (size_t)round_up(a.K, BIG_K) * (size_t)round_up(a.N, bn) * 2 : 0;
 }
 int launch_fc_nt(int type, const FcNtArgs &a, void *ws, hipStream_t st) {
-    if (big_fits(type, a)) return type == PS_T_BF16 ? nt_big<__bf16>(a, ws, st) : nt_big<_Float16>(a, ws, st);
+    const int bn = big_tile(type, a);
+    if (bn == 256) return type == PS_T_BF16 ? nt_big<__bf16, 256>(a, ws, st) : nt_big<_Float16, 256>(a, ws, st);
+    if (bn == 128) return type == PS_T_BF16 ? nt_big<__bf16, 128>(a, ws, st) : nt_big<_Float16, 128>(a, ws, st);
     return type == PS_T_F32 ? nt_t<float>(a, st) : type == PS_T_BF16 ? nt_t<__bf16>(a, st) : nt_t<_Float16>(a, st);
 }
 int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st) {
