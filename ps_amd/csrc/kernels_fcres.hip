@@ -524,7 +524,7 @@ __global__ __launch_bounds__(256) void k_fc_tn(FcTnArgs a, int tiles_n, int tile
         if (s + 1 < s_hi) put(buf ^ 1);
         __syncthreads();
     }
-    float *part = a.part + (size_t)split * (size_t)(a.K + 1) * a.N;
+    float *part = a.part + (size_t)split * (size_t)(a.K + a.nbias) * a.N;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
         const int n = n0 + wn + j * TILE + lr;
@@ -538,6 +538,160 @@ __global__ __launch_bounds__(256) void k_fc_tn(FcTnArgs a, int tiles_n, int tile
             }
         if (do_bias && lg == 0) part[(size_t)a.K * a.N + n] = accb[j][0];
     }
+}
+
+// x^T dz, 16-bit: the same machine as k_fc_nt_big with the batch as the sum's axis, 256 x 256 of dW per workgroup over one part of the
+// batch.  A step is 64 rows of both operands; a quarter holds their columns 128 h .. 128 h + 127, so its rows are 256 contiguous bytes.
+// Fragments need 8 values down a column: two transposing LDS reads (16 lanes read 4 rows x 16 columns and get a column's 4 rows each;
+// both operands take the batch in the same order, which is all the sum needs).  32-byte pieces are exchanged by the row's low 3 bits,
+// which are the lane's own, the same in every read.
+// db is dz times a fragment of ones: every workgroup of a row of tiles, and of it one of the two wave rows, takes its share of the
+// steps, so that no workgroup is the slow one; each leaves its own row behind dW's in the slab.
+// Columns behind K and N, and rows behind the part's last, are sent out of the buffer's bounds: zeros.
+template <typename T>
+__global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, int tiles_n) {
+    typedef Mma<T> X;
+    typedef typename X::frag frag;
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    constexpr int Q = 64 * 16;
+    constexpr int OX[2] = {0, 3 * Q}, OW[2] = {Q, 2 * Q};
+    __shared__ u32x4 lds[2][4 * Q];              // [step][x0 | w0 | w1 | x1] (w: dz)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+    const bool second = wave >= 4;
+    const int tiles = tiles_k * tiles_n, id = xcd_tile(blockIdx.x, gridDim.x), split = id / tiles, tile = id % tiles;
+    const int kt = tile / tiles_n, k0 = kt * 256, n0 = (tile % tiles_n) * 256;
+    const int64_t all = ((int64_t)a.M + 63) / 64, s_lo = all * split / a.nsplit, s_hi = all * (split + 1) / a.nsplit;
+    const int64_t m_lo = s_lo * 64, m_hi = s_hi * 64 < a.M ? s_hi * 64 : a.M;
+    const int steps = (int)(s_hi - s_lo), tail = (int)(m_hi - m_lo) - (steps - 1) * 64;      // rows of the last step
+    const auto rsX = __builtin_amdgcn_make_buffer_rsrc((void *)((const T *)a.X + m_lo * a.ldx), 0, (int)(((m_hi - m_lo - 1) * a.ldx + a.K) * 2), 0x00020000);
+    const auto rsW = __builtin_amdgcn_make_buffer_rsrc((void *)((const T *)a.D + m_lo * a.ldd), 0, (int)(((m_hi - m_lo - 1) * a.ldd + a.N) * 2), 0x00020000);
+    // piece tid of the first 32 rows of a quarter and of the second: row tid / 16 (+ 32), its 16 bytes exchanged within the row
+    const int row = tid >> 4, col = ((((tid & 15) >> 1) ^ (row & 7)) * 2 + (tid & 1)) * 8;
+    constexpr int OUT = 0x7ffffff0;
+    int vx[2], vw[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        vx[h] = k0 + h * 128 + col < a.K ? (int)(row * a.ldx + k0 + h * 128 + col) * 2 : OUT;
+        vw[h] = n0 + h * 128 + col < a.N ? (int)(row * a.ldd + n0 + h * 128 + col) * 2 : OUT;
+    }
+    const int sx = (int)a.ldx * 64, sw = (int)a.ldd * 64;                    // bytes of 32 rows
+    auto ask = [&](int t, const __amdgpu_buffer_rsrc_t &rs, int v, int s32, int at) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int vv = t == steps - 1 && row + i * 32 >= tail ? OUT : v;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)&lds[t & 1][at + i * 512 + wave * 64], 16, vv, (2 * t + i) * s32, 0, 0);
+        }
+    };
+    auto ask_x = [&](int t, int half) { ask(t, rsX, vx[half], sx, OX[half]); };
+    auto ask_w = [&](int t, int half) { ask(t, rsW, vw[half], sw, OW[half]); };
+    f32x4 acc[4][8], accb[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        accb[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int lr = lane & 15, lg = lane >> 4, key = (lg & 1) * 4 + (lr >> 2), lo = (lg * 4 + (lr >> 2)) * 128 + (lr & 3) * 4;
+    int ox[4], ow[2];                            // in 16-bit values
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ox[j] = lo + ((wm * 4 + j) ^ key) * 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ow[i] = lo + ((wn * 2 + i) ^ key) * 16;
+    frag fx[2][4], fw[2][4], ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = (T)1.f;
+    auto column = [&](const short *base, int k) {
+        union { frag f; s16x4 h[2]; } u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(base + (k * 32 + h * 16) * 128));
+        return u.f;
+    };
+    auto read_x = [&](int t, int half) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fx[k][j] = column((const short *)&lds[t & 1][OX[half]] + ox[j], k);
+    };
+    auto read_w = [&](int t, int half) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) fw[k][half * 2 + i] = column((const short *)&lds[t & 1][OW[half]] + ow[i], k);
+    };
+    auto multiply = [&](int hx, int hw) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) acc[hw * 2 + i][hx * 4 + j] = X::mma(fw[k][hw * 2 + i], fx[k][j], acc[hw * 2 + i][hx * 4 + j]);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto turn = [&]() { __builtin_amdgcn_sched_barrier(0); __builtin_amdgcn_s_barrier(); __builtin_amdgcn_sched_barrier(0); };
+    int next_b = kt * 2 + wm;                    // the next step whose dz this wave adds up
+    auto add_up = [&](int t, int hw) {
+        if (t != next_b) return;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) accb[hw * 2 + i] = X::mma(fw[k][hw * 2 + i], ones, accb[hw * 2 + i]);
+        if (hw == 1) next_b += 2 * tiles_k;
+    };
+    ask_x(0, 0); ask_w(0, 0); ask_w(0, 1); ask_x(0, 1);
+    if (steps > 1) {
+        ask_x(1, 0); ask_w(1, 0); ask_w(1, 1);
+        PS_WAIT_LOADS(10);
+    } else {
+        PS_WAIT_LOADS(0);
+    }
+    turn();
+    if (second) turn();
+    int t = 0;
+    for (; t < steps - 2; ++t) {
+        read_x(t, 0); read_w(t, 0); ask_x(t + 1, 1);
+        PS_WAIT_LOADS(10); turn(); multiply(0, 0); add_up(t, 0); turn();
+        read_w(t, 1); ask_x(t + 2, 0);
+        PS_WAIT_LOADS(10); turn(); multiply(0, 1); add_up(t, 1); turn();
+        read_x(t, 1); ask_w(t + 2, 0);
+        PS_WAIT_LOADS(10); turn(); multiply(1, 1); turn();
+        ask_w(t + 2, 1);
+        PS_WAIT_LOADS(10); turn(); multiply(1, 0); turn();
+    }
+    for (; t < steps; ++t) {
+        read_x(t, 0); read_w(t, 0);
+        if (t + 1 < steps) ask_x(t + 1, 1);
+        PS_WAIT_LOADS(0); turn(); multiply(0, 0); add_up(t, 0); turn();
+        read_w(t, 1);
+        PS_WAIT_LOADS(0); turn(); multiply(0, 1); add_up(t, 1); turn();
+        read_x(t, 1);
+        PS_WAIT_LOADS(0); turn(); multiply(1, 1); turn();
+        turn(); multiply(1, 0); turn();
+    }
+    if (!second) turn();
+    float *part = a.part + (size_t)split * (size_t)(a.K + a.nbias) * a.N;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = n0 + (i >> 1) * 128 + wn * 32 + (i & 1) * 16 + lg * 4;
+        if (n >= a.N) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = k0 + (j >> 2) * 128 + wm * 64 + (j & 3) * 16 + lr;
+            if (k < a.K) *reinterpret_cast<f32x4 *>(part + (size_t)k * a.N + n) = acc[i][j];
+        }
+        if (lr == 0) *reinterpret_cast<f32x4 *>(part + (size_t)(a.K + kt * 2 + wm) * a.N + n) = accb[i];
+    }
+}
+
+__global__ __launch_bounds__(256) void k_fc_grad_reduce(FcTnArgs a, float *__restrict__ dst, int accum) {
+    const int64_t n = (int64_t)a.K * a.N, i = (int64_t)blockIdx.x * 256 + threadIdx.x, slab = (int64_t)(a.K + a.nbias) * a.N;
+    if (i >= n + a.N) return;
+    const int rows = i < n ? 1 : a.nbias;
+    float s = 0.f;
+    for (int z = 0; z < a.nsplit; ++z)
+        for (int r = 0; r < rows; ++r) s += a.part[z * slab + i + (int64_t)r * a.N];
+    s /= (float)a.M;
+    dst[i] = accum ? dst[i] + s : s;
 }
 
 int grid_ok(int64_t blocks) {
@@ -582,6 +736,14 @@ template <typename T> int tn_t(const FcTnArgs &a, hipStream_t st) {
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
+template <typename T> int tn_big(const FcTnArgs &a, hipStream_t st) {
+    const int tiles_n = cdiv(a.N, 256), tiles_k = cdiv(a.K, 256);
+    const int64_t blocks = (int64_t)tiles_n * tiles_k * a.nsplit;
+    PSCHK(grid_ok(2 * blocks));
+    hipLaunchKernelGGL((k_fc_tn_big<T>), dim3((unsigned)blocks), dim3(512), 0, st, a, tiles_k, tiles_n);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
+}
 template <typename T>
 int ag_t(int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st) {
     const int64_t blocks = ((int64_t)cdiv(N, Chunk<T>::N) * M + 255) / 256;
@@ -608,12 +770,32 @@ int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void 
            : type == PS_T_BF16 ? ag_t<__bf16>(act, dy, lddy, z, ldz, dz, lddz, M, N, st)
                                : ag_t<_Float16>(act, dy, lddy, z, ldz, dz, lddz, M, N, st);
 }
-int fc_tn_splits(int type, int M, int K, int N) {
-    const int64_t tiles = (int64_t)cdiv(N, 128) * cdiv(K, 128), steps = cdiv(M, type == PS_T_F32 ? 32 : 64);
+// How dW is taken apart: a.big, a.nsplit, a.nbias.  The large tiles want 16-byte pieces, offsets of 31 bits inside a part, and parts of at
+// least 16 steps; one workgroup for each of the 256 CUs.
+void fc_tn_plan(int type, FcTnArgs &a) {
+    const bool f32 = type == PS_T_F32;
+    const int64_t big = (int64_t)cdiv(a.N, 256) * cdiv(a.K, 256), steps = cdiv(a.M, 64);
+    a.big = 0;
+    if (!f32 && !((uintptr_t)a.X % 16 || (uintptr_t)a.D % 16 || a.ldx % 8 || a.ldd % 8 || a.K % 8 || a.N % 8) && big * steps >= 2048) {
+        int64_t s = big >= 256 ? 1 : 256 / big;
+        if (s > steps / 16) s = steps / 16 > 0 ? steps / 16 : 1;
+        const int64_t rows = (cdiv(steps, s) + 1) * 64, ld = a.ldx > a.ldd ? a.ldx : a.ldd;
+        if (rows * ld * 2 < (1ll << 31) - 64) { a.big = 1; a.nsplit = (int)s; a.nbias = 2 * cdiv(a.K, 256); return; }
+    }
+    const int64_t tiles = (int64_t)cdiv(a.N, 128) * cdiv(a.K, 128), st = cdiv(a.M, f32 ? 32 : 64);
     int64_t s = (512 + tiles - 1) / tiles;               // two workgroups for each of the 256 CUs
-    if (s > steps / 4) s = steps / 4;                    // and no part shorter than four steps
-    return (int)(s < 1 ? 1 : s);
+    if (s > st / 4) s = st / 4;                          // and no part shorter than four steps
+    a.nsplit = (int)(s < 1 ? 1 : s); a.nbias = 1;
 }
 int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st) {
+    if (a.big) return type == PS_T_BF16 ? tn_big<__bf16>(a, st) : tn_big<_Float16>(a, st);
     return type == PS_T_F32 ? tn_t<float>(a, st) : type == PS_T_BF16 ? tn_t<__bf16>(a, st) : tn_t<_Float16>(a, st);
+}
+// The slabs' sum and mean: dW's rows over the parts, db's over the parts and their rows 
+int launch_fc_grad_reduce(const FcTnArgs &a, float *dst, int accum, hipStream_t st) {
+    const int64_t n = (int64_t)(a.K + 1) * a.N;
+    PSCHK(grid_ok((n + 255) / 256));
+    hipLaunchKernelGGL(k_fc_grad_reduce, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, dst, accum);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
 }

@@ -41,15 +41,17 @@ size_t fc_nt_workspace(int type, const FcNtArgs &a);                        // b
 int launch_fc_nt(int type, const FcNtArgs &a, void *ws, hipStream_t st);
 // dz = dy * act'(z), rounded to the type; rows of lddz elements
 int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st);
-// part[s][k][n] = sum over the s-th part of m of X[m][k] * D[m][n], k < K; row K: the sum of D[m][n]
+// part[s][k][n] = sum over the s-th part of m of X[m][k] * D[m][n], k < K; the nbias rows behind: shares of the sum of D[m][n]
 struct FcTnArgs {
     const void *X; int64_t ldx;
     const void *D; int64_t ldd;
-    float *part;                       // [nsplit][K + 1][N]
-    int M, K, N, nsplit;
+    float *part;                       // [nsplit][K + nbias][N]
+    int M, K, N;
+    int big, nsplit, nbias;            // filled by fc_tn_plan
 };
-int fc_tn_splits(int type, int M, int K, int N);
+void fc_tn_plan(int type, FcTnArgs &a);
 int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st);
+int launch_fc_grad_reduce(const FcTnArgs &a, float *dst, int accum, hipStream_t st);      // [K + 1][N]: means over M
 
 #ifdef __HIPCC__
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));

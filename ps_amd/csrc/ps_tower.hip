@@ -237,24 +237,25 @@ extern "C" int ps_fc_res_backward(ps_store_t *s, int layer, int type, int act, c
     int accum;
     PSCHK(grad_target(s, *p, grad_dev, &dst, &accum));
     // workspace: [slabs of dW | db][dz][what the product for dx needs]
-    const int nsplit = fc_tn_splits(type, B, K, N);
-    const int64_t slab = (int64_t)(K + 1) * N, lddz = round_up(N, 8);
-    const size_t slabs = (size_t)round_up((int64_t)sizeof(float) * slab * nsplit, 256), dzs = z_dev ? (size_t)round_up(es * lddz * B, 256) : 0;
+    const int64_t lddz = round_up(N, 8);
+    FcTnArgs t;
+    t.X = x_dev; t.ldx = ldx; t.D = z_dev ? nullptr : dy_dev; t.ldd = z_dev ? lddz : lddy; t.M = B; t.K = K; t.N = N;      // (dz: 256-byte aligned in the workspace)
+    fc_tn_plan(type, t);
+    const size_t slabs = (size_t)round_up((int64_t)sizeof(float) * (K + t.nbias) * N * t.nsplit, 256), dzs = z_dev ? (size_t)round_up(es * lddz * B, 256) : 0;
     FcNtArgs a;
     a.A = dy_dev; a.lda = lddy; a.W = p->W; a.ldw = p->ldw; a.bias = nullptr; a.R = skip_dev; a.ldr = skip_dev ? ldskip : 0; a.Z = nullptr; a.ldz = 0;
     a.Y = dx_dev; a.ldy = lddx; a.M = B; a.N = K; a.K = N; a.act = PS_ACT_NONE;
-    if (z_dev) { a.A = nullptr; a.lda = lddz; }             // (dz: 256-byte aligned in the workspace)
+    if (z_dev) { a.A = nullptr; a.lda = lddz; }
     char *ws;
     PSCHK(workspace(s, slabs + dzs + (dx_dev ? fc_nt_workspace(type, a) : 0), &ws));
+    t.part = (float *)ws;
     if (z_dev) {
-        a.A = ws + slabs;
+        t.D = a.A = ws + slabs;
         PSCHK(launch_act_grad(type, act, dy_dev, lddy, z_dev, ldz, ws + slabs, lddz, B, N, st));
     }
     if (dx_dev) PSCHK(launch_fc_nt(type, a, ws + slabs + dzs, st));
-    FcTnArgs t;
-    t.X = x_dev; t.ldx = ldx; t.D = a.A; t.ldd = a.lda; t.part = (float *)ws; t.M = B; t.K = K; t.N = N; t.nsplit = nsplit;
     PSCHK(launch_fc_tn(type, t, st));
-    PSCHK(launch_grad_reduce(t.part, nsplit, slab, slab, B, dst, accum, st));
+    PSCHK(launch_fc_grad_reduce(t, dst, accum, st));
     if (!grad_dev) p->pending_cnt++;
     return PS_OK;
 }
