@@ -5,71 +5,117 @@
 //             dx = skip + rstd * (p - mean(p) - h * mean(p * h)),   dgamma = sum_rows dy * h,   dbeta = sum_rows dy
 //
 // Both are bound by memory: a row is read once, lies in registers (as it came: 16 bits stay 16 bits) while its sums are formed in two
-// passes over them -- the variance from differences to the mean, never from sum x^2 -- and is written once.  All arithmetic is f32.
-// A row belongs to TPR lanes (4, 16, 64 of one wave, or a workgroup of 256) that hold NV 16-byte pieces each: a narrow row does not
-// idle a wave, a wide one does not spill.  Rows wider than 256 lanes x 32 elements take the kernels that walk the row again (from L2).
+// passes over them -- the variance from differences to the mean, never from sum x^2 -- and is written once; the next row's loads are in
+// flight meanwhile.  All arithmetic is f32.  A row belongs to TPR lanes (4, 16 or 64 of one wave, or a workgroup of 256 or 512) that
+// hold up to 16 elements each: a narrow row does not idle a wave, a wide one does not spill.  Rows wider than 8192 take the kernels
+// that walk the row again (from L2).  EDGE: the width is no multiple of a 16-byte piece, so the last piece is cut off element by element;
+// without it a lane behind the row's end reads the row's first piece and counts it as zeros, and no load hides behind a branch.
 #include "kernels_tower.h"
 
 namespace {
 
-constexpr int kMaxEpl = 32;            // elements of a row per lane
+constexpr int kMaxEpl = 16;            // elements of a row per lane
 
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float *lds) {
+// N sums over the TPR lanes of a row at once; slot: alternating, so that one barrier is enough
+template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float (*lds)[16][2], int &slot) {
 #pragma unroll
-    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    if (TPR > 64) {                    // the four waves of the workgroup, in wave order
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    if constexpr (TPR > 64) {          // the waves of the workgroup, in wave order
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) lds[slot][threadIdx.x >> 6][i] = v[i];
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = lds[slot][0][i];
+#pragma unroll
+            for (int w = 1; w < TPR / 64; ++w) v[i] += lds[slot][w][i];
+        }
+        slot ^= 1;
     }
-    return v;
+}
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float (*lds)[16][2], int &slot) {
+    float s[1] = {v};
+    row_sums<TPR, 1>(s, lds, slot);
+    return s[0];
 }
 
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(256) void k_ln_fwd(LnFwdArgs a) {
-    constexpr int VEC = Chunk<T>::N, RPB = 256 / TPR;
-    __shared__ float lds[4];
-    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-    const float inv_d = 1.f / (float)a.D;
-    float g[NV * VEC], b[NV * VEC];
+template <typename T, int TPR, int NV, bool EDGE> struct RowPieces {
+    static constexpr int VEC = Chunk<T>::N;
+    Chunk<T> c[NV];
+    __device__ __forceinline__ void load(const T *row, int t, int D) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = (t + i * TPR) * VEC;
+            if constexpr (EDGE) c[i].load(row, e, D);
+            else c[i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(row + (e < D ? e : 0));
+        }
+    }
+    __device__ __forceinline__ void store(T *row, int t, int D) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = (t + i * TPR) * VEC;
+            if constexpr (EDGE) c[i].store(row, e, D);
+            else if (e < D) *reinterpret_cast<typename Chunk<T>::unaligned_t *>(row + e) = c[i].u;
+        }
+    }
+};
+// does element j of piece i lie in the row?
+template <int TPR, int VEC, bool EDGE> __device__ __forceinline__ bool inside(int t, int i, int j, int D) {
+    return (t + i * TPR) * VEC + (EDGE ? j : 0) < D;
+}
+template <typename T, int TPR, int NV> __device__ __forceinline__ void load_params(float (&p)[NV * Chunk<T>::N], const float *src, int t, int D) {
+    constexpr int VEC = Chunk<T>::N;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             const int c = (t + i * TPR) * VEC + j;
-            g[i * VEC + j] = c < a.D ? a.gamma[c] : 0.f;
-            b[i * VEC + j] = c < a.D ? a.beta[c] : 0.f;
+            p[i * VEC + j] = src[c < D ? c : 0];
         }
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.B; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t r = r0 + sub < a.B ? r0 + sub : a.B - 1;      // a lane group behind the last row repeats it and writes nothing
-        const T *x = (const T *)a.x + r * a.ldx;
-        Chunk<T> v[NV];
+}
+
+template <typename T, int TPR, int NV, bool EDGE>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_fwd(LnFwdArgs a) {
+    constexpr int VEC = Chunk<T>::N, RPB = TPR > 256 ? 1 : 256 / TPR;
+    __shared__ float lds[2][16][2];
+    int slot = 0;
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const float inv_d = 1.f / (float)a.D;
+    const int64_t stride = (int64_t)gridDim.x * RPB;
+    int64_t r = (int64_t)blockIdx.x * RPB + sub;
+    // a lane group behind the last row repeats it and writes nothing
+    RowPieces<T, TPR, NV, EDGE> v, next;
+    next.load((const T *)a.x + (r < a.B ? r : a.B - 1) * a.ldx, t, a.D);
+    float g[NV * VEC], b[NV * VEC];
+    load_params<T, TPR, NV>(g, a.gamma, t, a.D);
+    load_params<T, TPR, NV>(b, a.beta, t, a.D);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.B; r0 += stride, r += stride) {
+        v = next;
+        if (r0 + stride < a.B) next.load((const T *)a.x + (r + stride < a.B ? r + stride : a.B - 1) * a.ldx, t, a.D);
         float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) v[i].load(x, (t + i * TPR) * VEC, a.D);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s += (float)v[i].e[j];
-        const float mean = row_sum<TPR>(s, lds) * inv_d;
+            for (int j = 0; j < VEC; ++j) s += inside<TPR, VEC, EDGE>(t, i, j, a.D) ? (float)v.c[i].e[j] : 0.f;
+        const float mean = row_sum<TPR>(s, lds, slot) * inv_d;
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float d = (t + i * TPR) * VEC + j < a.D ? (float)v[i].e[j] - mean : 0.f;
+                const float d = inside<TPR, VEC, EDGE>(t, i, j, a.D) ? (float)v.c[i].e[j] - mean : 0.f;
                 s = fmaf(d, d, s);
             }
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(s, lds) * inv_d + a.eps);
-        if (r0 + sub >= a.B) continue;
-        T *y = (T *)a.y + r * a.ldy;
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(s, lds, slot) * inv_d + a.eps);
+        if (r >= a.B) continue;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i].e[j] = (T)fmaf(((float)v[i].e[j] - mean) * rstd, g[i * VEC + j], b[i * VEC + j]);
-            v[i].store(y, (t + i * TPR) * VEC, a.D);
-        }
+            for (int j = 0; j < VEC; ++j) v.c[i].e[j] = (T)fmaf(((float)v.c[i].e[j] - mean) * rstd, g[i * VEC + j], b[i * VEC + j]);
+        v.store((T *)a.y + r * a.ldy, t, a.D);
         if (a.stats && t == 0) { a.stats[2 * r] = mean; a.stats[2 * r + 1] = rstd; }
     }
 }
@@ -78,7 +124,8 @@ __global__ __launch_bounds__(256) void k_ln_fwd(LnFwdArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_ln_fwd_wide(LnFwdArgs a) {
     constexpr int VEC = Chunk<T>::N;
-    __shared__ float lds[4];
+    __shared__ float lds[2][16][2];
+    int slot = 0;
     const float inv_d = 1.f / (float)a.D;
     for (int64_t r = blockIdx.x; r < a.B; r += gridDim.x) {
         const T *x = (const T *)a.x + r * a.ldx;
@@ -90,7 +137,7 @@ __global__ __launch_bounds__(256) void k_ln_fwd_wide(LnFwdArgs a) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) s += (float)v.e[j];
         }
-        const float mean = row_sum<256>(s, lds) * inv_d;
+        const float mean = row_sum<256>(s, lds, slot) * inv_d;
         s = 0.f;
         for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.D; c += 256 * VEC) {
             v.load(x, (int)c, a.D);
@@ -100,7 +147,7 @@ __global__ __launch_bounds__(256) void k_ln_fwd_wide(LnFwdArgs a) {
                 s = fmaf(d, d, s);
             }
         }
-        const float rstd = 1.f / sqrtf(row_sum<256>(s, lds) * inv_d + a.eps);
+        const float rstd = 1.f / sqrtf(row_sum<256>(s, lds, slot) * inv_d + a.eps);
         for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.D; c += 256 * VEC) {
             v.load(x, (int)c, a.D);
 #pragma unroll
@@ -114,78 +161,80 @@ __global__ __launch_bounds__(256) void k_ln_fwd_wide(LnFwdArgs a) {
 
 // Every lane keeps the column sums of its own columns over all the rows it sees; a workgroup folds its RPB row groups through LDS and
 // writes one slab: no atomics, the same order in every run.
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(256) void k_ln_bwd(LnBwdArgs a) {
-    constexpr int VEC = Chunk<T>::N, RPB = 256 / TPR, E = NV * VEC;
-    __shared__ float lds[4];
-    __shared__ float fold[RPB > 1 ? 256 * VEC : 1];
+template <typename T, int TPR, int NV, bool EDGE>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_bwd(LnBwdArgs a) {
+    constexpr int VEC = Chunk<T>::N, RPB = TPR > 256 ? 1 : 256 / TPR, E = NV * VEC;
+    __shared__ float lds[2][16][2];
+    __shared__ float fold[TPR < 256 ? 4 * (TPR < 64 ? TPR : 64) * VEC : 1];
+    int slot = 0;
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const float inv_d = 1.f / (float)a.D;
+    const int64_t stride = (int64_t)gridDim.x * RPB;
+    int64_t r = (int64_t)blockIdx.x * RPB + sub;
+    RowPieces<T, TPR, NV, EDGE> x, dy, k, nx, ndy, nk;
+    float mean, rstd, nmean, nrstd;
+    auto fetch = [&](int64_t q) {
+        if (q >= a.B) q = a.B - 1;
+        nx.load((const T *)a.x + q * a.ldx, t, a.D);
+        ndy.load((const T *)a.dy + q * a.lddy, t, a.D);
+        if (a.skip) nk.load((const T *)a.skip + q * a.ldskip, t, a.D);
+        nmean = a.stats[2 * q]; nrstd = a.stats[2 * q + 1];
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) nk.c[i].zero();
+    fetch(r);
     float g[E], sg[E], sb[E];
+    load_params<T, TPR, NV>(g, a.gamma, t, a.D);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const int c = (t + i * TPR) * VEC + j;
-            g[i * VEC + j] = c < a.D ? a.gamma[c] : 0.f;
-            sg[i * VEC + j] = 0.f; sb[i * VEC + j] = 0.f;
-        }
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.B; r0 += (int64_t)gridDim.x * RPB) {
-        const bool live = r0 + sub < a.B;
-        const int64_t r = live ? r0 + sub : a.B - 1;
-        const T *x = (const T *)a.x + r * a.ldx, *dy = (const T *)a.dy + r * a.lddy;
-        Chunk<T> v[NV], w[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) { v[i].load(x, (t + i * TPR) * VEC, a.D); w[i].load(dy, (t + i * TPR) * VEC, a.D); }
-        const float mean = a.stats[2 * r], rstd = a.stats[2 * r + 1];
-        float s1 = 0.f, s2 = 0.f;
+    for (int i = 0; i < E; ++i) { sg[i] = 0.f; sb[i] = 0.f; }
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.B; r0 += stride, r += stride) {
+        const bool live = r < a.B;
+        x = nx; dy = ndy; k = nk; mean = nmean; rstd = nrstd;
+        if (r0 + stride < a.B) fetch(r + stride);
+        float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const bool in = live && (t + i * TPR) * VEC + j < a.D;
-                const float h = in ? ((float)v[i].e[j] - mean) * rstd : 0.f, d = in ? (float)w[i].e[j] : 0.f, p = d * g[i * VEC + j];
-                s1 += p; s2 = fmaf(p, h, s2);
+                const bool in = live && inside<TPR, VEC, EDGE>(t, i, j, a.D);
+                const float h = in ? ((float)x.c[i].e[j] - mean) * rstd : 0.f, d = in ? (float)dy.c[i].e[j] : 0.f, p = d * g[i * VEC + j];
+                s[0] += p; s[1] = fmaf(p, h, s[1]);
                 sg[i * VEC + j] = fmaf(d, h, sg[i * VEC + j]); sb[i * VEC + j] += d;
             }
         if (!a.dx) continue;
-        const float m1 = row_sum<TPR>(s1, lds) * inv_d, m2 = row_sum<TPR>(s2, lds) * inv_d;
+        row_sums<TPR, 2>(s, lds, slot);
         if (!live) continue;
-        T *dx = (T *)a.dx + r * a.lddx;
-        const T *sk = (const T *)a.skip + r * a.ldskip;
+        const float m1 = s[0] * inv_d, m2 = s[1] * inv_d;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (t + i * TPR) * VEC;
-            Chunk<T> k;
-            k.zero();
-            if (a.skip) k.load(sk, c, a.D);
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float h = ((float)v[i].e[j] - mean) * rstd, p = (float)w[i].e[j] * g[i * VEC + j];
-                k.e[j] = (T)((float)k.e[j] + rstd * (p - m1 - h * m2));
+                const float h = ((float)x.c[i].e[j] - mean) * rstd, p = (float)dy.c[i].e[j] * g[i * VEC + j];
+                k.c[i].e[j] = (T)((float)k.c[i].e[j] + rstd * (p - m1 - h * m2));
             }
-            k.store(dx, c, a.D);
-        }
+        k.store((T *)a.dx + r * a.lddx, t, a.D);
     }
     float *out = a.part + (size_t)blockIdx.x * 2 * a.D;
+#pragma unroll
     for (int w = 0; w < 2; ++w) {
         float *acc = w ? sb : sg;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (RPB > 1) {
-                __syncthreads();
+            if constexpr (TPR < 256) {           // the row groups of a wave lane by lane, then the four waves through LDS
+                constexpr int L = TPR < 64 ? TPR : 64;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) fold[threadIdx.x * VEC + j] = acc[i * VEC + j];
-                __syncthreads();
-                if (sub == 0) {
+                for (int j = 0; j < VEC; ++j)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        float s = fold[t * VEC + j];
-#pragma unroll 1
-                        for (int q = 1; q < RPB; ++q) s += fold[(q * TPR + t) * VEC + j];
-                        acc[i * VEC + j] = s;
-                    }
-                }
+                    for (int o = TPR; o < 64; o <<= 1) acc[i * VEC + j] += __shfl_xor(acc[i * VEC + j], o);
+                __syncthreads();
+                if ((threadIdx.x & 63) < L)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) fold[((threadIdx.x >> 6) * L + t) * VEC + j] = acc[i * VEC + j];
+                __syncthreads();
+                if (sub == 0)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        acc[i * VEC + j] = (fold[t * VEC + j] + fold[(L + t) * VEC + j]) + (fold[(2 * L + t) * VEC + j] + fold[(3 * L + t) * VEC + j]);
             }
             if (sub == 0) {
 #pragma unroll
@@ -202,7 +251,8 @@ __global__ __launch_bounds__(256) void k_ln_bwd(LnBwdArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_ln_bwd_wide(LnBwdArgs a) {
     constexpr int VEC = Chunk<T>::N;
-    __shared__ float lds[4];
+    __shared__ float lds[2][16][2];
+    int slot = 0;
     const float inv_d = 1.f / (float)a.D;
     float *sg = a.part + (size_t)blockIdx.x * 2 * a.D, *sb = sg + a.D;
     for (int64_t r = blockIdx.x; r < a.B; r += gridDim.x) {
@@ -223,7 +273,7 @@ __global__ __launch_bounds__(256) void k_ln_bwd_wide(LnBwdArgs a) {
                 }
         }
         if (!a.dx) continue;
-        const float m1 = row_sum<256>(s1, lds) * inv_d, m2 = row_sum<256>(s2, lds) * inv_d;
+        const float m1 = row_sum<256>(s1, lds, slot) * inv_d, m2 = row_sum<256>(s2, lds, slot) * inv_d;
         T *dx = (T *)a.dx + r * a.lddx;
         for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.D; c += 256 * VEC) {
             v.load(x, (int)c, a.D); w.load(dy, (int)c, a.D);
@@ -240,12 +290,24 @@ __global__ __launch_bounds__(256) void k_ln_bwd_wide(LnBwdArgs a) {
     }
 }
 
-__global__ __launch_bounds__(256) void k_grad_reduce(const float *__restrict__ part, int nslab, int64_t stride, int64_t n, int B,
-                                                     float *__restrict__ dst, int accum) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
+// 64 columns a workgroup; its 16 waves take the slabs in turn, 8 loads in flight each, and are added in wave order
+__global__ __launch_bounds__(1024) void k_grad_reduce(const float *__restrict__ part, int nslab, int64_t n, int B, float *__restrict__ dst, int accum) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i = (int64_t)blockIdx.x * 64 + lane, ic = i < n ? i : n - 1;
     float s = 0.f;
-    for (int z = 0; z < nslab; ++z) s += part[(size_t)z * stride + i];
+    for (int z0 = wave; z0 < nslab; z0 += 128) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = z0 + q * 16 < nslab ? part[(int64_t)(z0 + q * 16) * n + ic] : 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s += v[q];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave || i >= n) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += sums[w][lane];
     s /= (float)B;
     dst[i] = accum ? dst[i] + s : s;
 }
@@ -254,47 +316,46 @@ __global__ __launch_bounds__(256) void k_grad_reduce(const float *__restrict__ p
 struct Layout { int tpr, nv; };
 Layout layout_of(int vec, int D) {
     const int chunks = (D + vec - 1) / vec;
-    const int tprs[4] = {4, 16, 64, 256};
-    for (int i = 0; i < 4; ++i) {
-        const int cap = tprs[i] < 64 ? 2 : kMaxEpl / vec;
-        if (chunks > tprs[i] * cap) continue;
+    for (int tpr : {4, 16, 64, 256, 512}) {
+        if (chunks > tpr * (kMaxEpl / vec)) continue;
         int nv = 1;
-        while (tprs[i] * nv < chunks) nv *= 2;
-        return {tprs[i], nv};
+        while (tpr * nv < chunks) nv *= 2;
+        return {tpr, nv};
     }
     return {0, 0};
 }
 
 template <typename T, int TPR, int NV>
 int fwd_go(const LnFwdArgs &a, hipStream_t st) {
-    const int64_t need = ((int64_t)a.B + 256 / TPR - 1) / (256 / TPR);
-    hipLaunchKernelGGL((k_ln_fwd<T, TPR, NV>), dim3((unsigned)(need < 4096 ? need : 4096)), dim3(256), 0, st, a);
+    constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
+    const int64_t need = ((int64_t)a.B + RPB - 1) / RPB, most = TPR > 256 ? 512 : 2048;
+    const dim3 grid((unsigned)(need < most ? need : most)), block(TPR > 256 ? TPR : 256);
+    if (a.D % Chunk<T>::N) hipLaunchKernelGGL((k_ln_fwd<T, TPR, NV, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_ln_fwd<T, TPR, NV, false>), grid, block, 0, st, a);
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
 template <typename T, int TPR, int NV>
 int bwd_go(const LnBwdArgs &a, int nblk, hipStream_t st) {
-    hipLaunchKernelGGL((k_ln_bwd<T, TPR, NV>), dim3((unsigned)nblk), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)nblk), block(TPR > 256 ? TPR : 256);
+    if (a.D % Chunk<T>::N) hipLaunchKernelGGL((k_ln_bwd<T, TPR, NV, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_ln_bwd<T, TPR, NV, false>), grid, block, 0, st, a);
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
-// every (lanes, pieces) that layout_of can return for the type; NV 8 holds 32 elements only for f32
-#define LN_DISPATCH(GO, ...)                                                                                   \
-    switch (l.tpr * 16 + l.nv) {                                                                               \
-    case 4 * 16 + 1: return GO<T, 4, 1>(__VA_ARGS__);                                                          \
-    case 4 * 16 + 2: return GO<T, 4, 2>(__VA_ARGS__);                                                          \
-    case 16 * 16 + 1: return GO<T, 16, 1>(__VA_ARGS__);                                                        \
-    case 16 * 16 + 2: return GO<T, 16, 2>(__VA_ARGS__);                                                        \
-    case 64 * 16 + 1: return GO<T, 64, 1>(__VA_ARGS__);                                                        \
-    case 64 * 16 + 2: return GO<T, 64, 2>(__VA_ARGS__);                                                        \
-    case 64 * 16 + 4: return GO<T, 64, 4>(__VA_ARGS__);                                                        \
-    case 256 * 16 + 2: return GO<T, 256, 2>(__VA_ARGS__);                                                      \
-    case 256 * 16 + 4: return GO<T, 256, 4>(__VA_ARGS__);                                                      \
-    }                                                                                                          \
-    if constexpr (sizeof(T) == 4) {                                                                            \
-        if (l.tpr == 64 && l.nv == 8) return GO<T, 64, 8>(__VA_ARGS__);                                        \
-        if (l.tpr == 256 && l.nv == 8) return GO<T, 256, 8>(__VA_ARGS__);                                      \
+// every (lanes, pieces) that layout_of can return for the type: a wider group takes over where two pieces (f32: four) do not do
+#define LN_ROW(TPR, GO, ...)                                                                                   \
+    if (l.tpr == TPR) {                                                                                        \
+        if (l.nv == 1) return GO<T, TPR, 1>(__VA_ARGS__);                                                      \
+        if (l.nv == 2) return GO<T, TPR, 2>(__VA_ARGS__);                                                      \
+        if constexpr (sizeof(T) == 4) return GO<T, TPR, 4>(__VA_ARGS__);                                       \
     }
+#define LN_DISPATCH(GO, ...)                                                                                   \
+    LN_ROW(4, GO, __VA_ARGS__)                                                                                 \
+    LN_ROW(16, GO, __VA_ARGS__)                                                                                \
+    LN_ROW(64, GO, __VA_ARGS__)                                                                                \
+    LN_ROW(256, GO, __VA_ARGS__)                                                                               \
+    LN_ROW(512, GO, __VA_ARGS__)
 
 template <typename T> int fwd_t(const LnFwdArgs &a, hipStream_t st) {
     const Layout l = layout_of(Chunk<T>::N, a.D);
@@ -316,17 +377,19 @@ template <typename T> int bwd_t(const LnBwdArgs &a, int nblk, hipStream_t st) {
 int launch_ln_fwd(int type, const LnFwdArgs &a, hipStream_t st) {
     return type == PS_T_F32 ? fwd_t<float>(a, st) : type == PS_T_BF16 ? fwd_t<__bf16>(a, st) : fwd_t<_Float16>(a, st);
 }
+// Two workgroups a CU: with prefetched rows that is bytes enough in flight, and every further workgroup is a slab more to fold, write and
+// add up (bf16, 65536 x 1024: 111 us with 512 workgroups, 130 with 768, 119 with 1024, 128 with 1536; f32, 65536 x 256: 56 / 75 / 77 / 95)
 int ln_bwd_blocks(int type, int B, int D) {
     const Layout l = layout_of(type == PS_T_F32 ? 4 : 8, D);
-    const int rpb = l.tpr ? 256 / l.tpr : 1;
-    const int64_t need = ((int64_t)B + rpb - 1) / rpb;
-    return (int)(need < 512 ? need : 512);
+    const int rpb = l.tpr && l.tpr < 256 ? 256 / l.tpr : 1;
+    const int64_t need = ((int64_t)B + rpb - 1) / rpb, most = l.tpr > 256 ? 256 : 512;
+    return (int)(need < most ? need : most);
 }
 int launch_ln_bwd(int type, const LnBwdArgs &a, int nblk, hipStream_t st) {
     return type == PS_T_F32 ? bwd_t<float>(a, nblk, st) : type == PS_T_BF16 ? bwd_t<__bf16>(a, nblk, st) : bwd_t<_Float16>(a, nblk, st);
 }
-int launch_grad_reduce(const float *part, int nslab, int64_t stride, int64_t n, int B, float *dst, int accum, hipStream_t st) {
-    hipLaunchKernelGGL(k_grad_reduce, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, nslab, stride, n, B, dst, accum);
+int launch_grad_reduce(const float *part, int nslab, int64_t n, int B, float *dst, int accum, hipStream_t st) {
+    hipLaunchKernelGGL(k_grad_reduce, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st, part, nslab, n, B, dst, accum);
     HIPCHK(hipGetLastError());
     return PS_OK;
 }

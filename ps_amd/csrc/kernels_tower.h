@@ -24,8 +24,8 @@ int launch_ln_fwd(int type, const LnFwdArgs &a, hipStream_t st);
 int ln_bwd_blocks(int type, int B, int D);             // workgroups (= slabs of part) of launch_ln_bwd
 int launch_ln_bwd(int type, const LnBwdArgs &a, int nblk, hipStream_t st);
 
-// dst[i] = (accum ? dst[i] : 0) + (sum over z of part[z * stride + i]) / B        (fixed order of z)
-int launch_grad_reduce(const float *part, int nslab, int64_t stride, int64_t n, int B, float *dst, int accum, hipStream_t st);
+// dst[i] = (accum ? dst[i] : 0) + (sum over z of part[z * n + i]) / B        (fixed order of z)
+int launch_grad_reduce(const float *part, int nslab, int64_t n, int B, float *dst, int accum, hipStream_t st);
 
 // Y[m][n] = act(sum_k A[m][k] * Wr[n][k] + bias[n]) + R[m][n], Z = the pre-activation; Wr f32, rounded to the activations' type on the way
 struct FcNtArgs {

@@ -155,7 +155,7 @@ extern "C" int ps_ln_backward(ps_store_t *s, int layer, int type, const void *x_
     a.x = x_dev; a.ldx = ldx; a.dy = dy_dev; a.lddy = lddy; a.skip = skip_dev; a.ldskip = skip_dev ? ldskip : 0; a.dx = dx_dev; a.lddx = lddx;
     a.gamma = p->W; a.stats = stats_dev; a.part = (float *)ws; a.B = B; a.D = D;
     PSCHK(launch_ln_bwd(type, a, nblk, s->stream));
-    PSCHK(launch_grad_reduce(a.part, nblk, 2ll * D, 2ll * D, B, dst, accum, s->stream));
+    PSCHK(launch_grad_reduce(a.part, nblk, 2ll * D, B, dst, accum, s->stream));
     if (!grad_dev) p->pending_cnt++;
     return PS_OK;
 }
