@@ -93,12 +93,48 @@ template <typename T> __device__ __forceinline__ void load_w(Chunk<T> &o, const 
     }
 }
 
+// ... as they come, and rounded when they go into LDS
+template <typename T> struct Weights {
+    f32x4 lo, hi;
+    __device__ __forceinline__ void load(const float *p) { lo = reinterpret_cast<const f32x4 *>(p)[0]; hi = reinterpret_cast<const f32x4 *>(p)[1]; }
+    __device__ __forceinline__ void load(const float *row, int c, int n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { lo[j] = c + j < n ? row[c + j] : 0.f; hi[j] = c + 4 + j < n ? row[c + 4 + j] : 0.f; }
+    }
+    __device__ __forceinline__ Chunk<T> rounded() const {
+        Chunk<T> o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { o.e[j] = (T)lo[j]; o.e[4 + j] = (T)hi[j]; }
+        return o;
+    }
+};
+template <> struct Weights<float> {
+    Chunk<float> w;
+    __device__ __forceinline__ void load(const float *p) { w.u = *reinterpret_cast<const u32x4 *>(p); }
+    __device__ __forceinline__ void load(const float *row, int c, int n) { w.load(row, c, n); }
+    __device__ __forceinline__ Chunk<float> rounded() const { return w; }
+};
+
+// A barrier that waits for this wave's LDS traffic and lets its memory loads fly on (the builtin, which the compiler's own wait counting
+// sees: behind waits written in assembly it took finished loads for pending ones and waited again where it hurt)
+#define PS_WAIT_COUNTS(vm) __builtin_amdgcn_s_waitcnt(((vm) & 15) | 0x70 | (((vm) >> 4) << 14))
+#define PS_ORDERED(x)                  \
+    do {                               \
+        asm volatile("" ::: "memory"); \
+        x;                             \
+        asm volatile("" ::: "memory"); \
+    } while (0)
+#define PS_WAIT_LDS() PS_ORDERED(PS_WAIT_COUNTS(63))
+#define PS_WAIT_LOADS(n) PS_ORDERED(PS_WAIT_COUNTS(n))      // all but the last n loads have landed, too
+#define PS_BARRIER() PS_ORDERED(__builtin_amdgcn_s_barrier())
+
 // One BM x BN tile of the output per workgroup of 4 waves (2 x 2).  LDS rows are 128 bytes of the sum's axis (BK elements), 16-byte
-// pieces exchanged by the row's low bits so that the fragment reads of 8 neighbouring rows touch all banks once.  The next step's
-// pieces travel in registers while this step multiplies; two LDS buffers, one barrier a step.
+// pieces exchanged by the row's low bits so that the fragment reads of 8 neighbouring rows touch all banks once.  The pieces of the
+// next AHEAD steps travel in registers while this step multiplies; two LDS buffers, one barrier a step (which waits for LDS alone, not for
+// the loads).
 // The product is formed transposed (weights as the first operand): a lane then holds 4 neighbouring columns of one row of y.
-template <typename T, int BM, int BN>
-__global__ __launch_bounds__(256) void k_fc_nt(FcNtArgs a, int tiles_n) {
+template <typename T, int BM, int BN, int AHEAD>
+__global__ __launch_bounds__(256, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a, int tiles_n) {
     typedef Mma<T> X;
     typedef typename X::frag frag;
     constexpr int CN = Chunk<T>::N, BK = X::BK, TILE = X::TILE, FM = BM / 2 / TILE, FN = BN / 2 / TILE, PA = BM * 8 / 256, PB = BN * 8 / 256;
@@ -124,18 +160,27 @@ __global__ __launch_bounds__(256) void k_fc_nt(FcNtArgs a, int tiles_n) {
         pb[i] = a.W + (size_t)n * a.ldw;
         dst_b[i] = row * 8 + (ch ^ (row & 7));
     }
-    Chunk<T> ra[PA], rb[PB];
-    auto fetch = [&](int k0) {
+    Chunk<T> ra[AHEAD][PA];
+    Weights<T> rb[AHEAD][PB];
+    auto fetch = [&](int set, int k0) {
+        const int k = k0 + ch * CN;
 #pragma unroll
-        for (int i = 0; i < PA; ++i) ra[i].load(pa[i], k0 + ch * CN, a.K);
+        for (int i = 0; i < PA; ++i) ra[set][i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(pa[i] + k);
 #pragma unroll
-        for (int i = 0; i < PB; ++i) load_w<T>(rb[i], pb[i], k0 + ch * CN, a.K);
+        for (int i = 0; i < PB; ++i) rb[set][i].load(pb[i] + k);
     };
-    auto put = [&](int buf) {
+    auto fetch_cut = [&](int k0) {
+        const int k = k0 + ch * CN;
 #pragma unroll
-        for (int i = 0; i < PA; ++i) sA[buf][dst_a[i]] = ra[i].u;
+        for (int i = 0; i < PA; ++i) ra[0][i].load(pa[i], k, a.K);
 #pragma unroll
-        for (int i = 0; i < PB; ++i) sB[buf][dst_b[i]] = rb[i].u;
+        for (int i = 0; i < PB; ++i) rb[0][i].load(pb[i], k, a.K);
+    };
+    auto put = [&](int set, int buf) {
+#pragma unroll
+        for (int i = 0; i < PA; ++i) sA[buf][dst_a[i]] = ra[set][i].u;
+#pragma unroll
+        for (int i = 0; i < PB; ++i) sB[buf][dst_b[i]] = rb[set][i].rounded().u;
     };
     typename X::acc acc[FN][FM];
 #pragma unroll
@@ -146,13 +191,7 @@ __global__ __launch_bounds__(256) void k_fc_nt(FcNtArgs a, int tiles_n) {
             for (int e = 0; e < (int)(sizeof(acc[0][0]) / 4); ++e) acc[i][j][e] = 0.f;
     const int lr = lane % TILE, lg = lane / TILE;
     constexpr int KS = 8 / (64 / TILE);          // fragment steps per LDS row
-    fetch(0);
-    put(0);
-    __syncthreads();
-    const int steps = (a.K + BK - 1) / BK;
-    for (int s = 0; s < steps; ++s) {
-        const int buf = s & 1;
-        if (s + 1 < steps) fetch((s + 1) * BK);
+    auto multiply = [&](int buf) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             frag fa[FM], fb[FN];
@@ -166,8 +205,30 @@ __global__ __launch_bounds__(256) void k_fc_nt(FcNtArgs a, int tiles_n) {
 #pragma unroll
                 for (int j = 0; j < FM; ++j) acc[i][j] = X::mma(fb[i], fa[j], acc[i][j]);
         }
-        if (s + 1 < steps) put(buf ^ 1);
-        __syncthreads();
+    };
+    // the step that K cuts off, if there is one, goes first: behind it no load hides behind a branch
+    const int full = a.K / BK, cut = a.K % BK ? 1 : 0, steps = full + cut;
+    if (cut) fetch_cut(full * BK); else fetch(0, 0);
+    if (!full) {                                 // nothing but the cut step
+        put(0, 0);
+        PS_WAIT_LDS(); PS_BARRIER();
+        multiply(0);
+    } else {
+        // step s + p lies in buffer p and the next ones in registers or on their way.  The last steps ask again for what is there: the
+        // loads are never behind a branch, so the waits know how many of them are younger than those they wait for.
+        auto ask = [&](int set, int step) { fetch(set, (step < steps ? step - cut : full - 1) * BK); };
+        auto half = [&](int s, int p) {
+            if (AHEAD > 1) ask(p, s + p + 2); else ask(0, s + p + 1);
+            multiply(p);
+            put(AHEAD > 1 ? p ^ 1 : 0, p ^ 1);
+            PS_WAIT_LDS(); PS_BARRIER();
+        };
+        if (AHEAD > 1) ask(1, 1);
+        put(0, 0);
+        PS_WAIT_LDS(); PS_BARRIER();
+        int s = 0;
+        for (; s + 2 <= steps; s += 2) { half(s, 0); half(s, 1); }
+        if (s < steps) half(s, 0);
     }
     // epilogue: groups of 4 neighbouring columns of one row
     constexpr int GR = (int)(sizeof(acc[0][0]) / 16);
@@ -182,20 +243,99 @@ __global__ __launch_bounds__(256) void k_fc_nt(FcNtArgs a, int tiles_n) {
 #pragma unroll
             for (int q = 0; q < GR; ++q) {
                 const int n = n0 + wn + i * TILE + q * 8 + lg * 4;
+                if (n >= a.N) continue;
                 float v[4];
+                Quad<T> o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e] + (a.bias && n + e < a.N ? a.bias[n + e] : 0.f);
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e] + (a.bias ? a.bias[n + e] : 0.f);      // (the bias row is padded to a multiple of 16)
                 if (a.Z) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n + e < a.N) zr[n + e] = (T)v[e];
+                    for (int e = 0; e < 4; ++e) o.e[e] = (T)v[e];
+                    o.store(zr, n, a.N);
                 }
                 act_apply(v, a.act);
+                if (a.R) {
+                    o.load(rr, n, a.N);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < a.N) y[n + e] = (T)(a.R ? v[e] + (float)rr[n + e] : v[e]);
+                    for (int e = 0; e < 4; ++e) v[e] += (float)o.e[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o.e[e] = (T)v[e];
+                o.store(y, n, a.N);
             }
     }
+}
+
+// Few rows (or few tiles): one workgroup of 16 waves per 16 columns and 16 FM rows.  The waves share out the sum in steps and take their
+// fragments straight from memory -- the weights in f32, rounded in registers, each read once per row of tiles -- so that a call is two
+// dependent trips to memory and not a chain of staged steps; their sums meet in LDS and are added in wave order.
+template <typename T> struct MmaFew {
+    static constexpr int KS = 32;
+    static __device__ __forceinline__ f32x4 mma(const Chunk<T> &a, const Chunk<T> &b, f32x4 c) {
+        typedef typename Mma<T>::frag frag;
+        return Mma<T>::mma(__builtin_bit_cast(frag, a.u), __builtin_bit_cast(frag, b.u), c);
+    }
+};
+template <> struct MmaFew<float> {
+    static constexpr int KS = 16;
+    static __device__ __forceinline__ f32x4 mma(const Chunk<float> &a, const Chunk<float> &b, f32x4 c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.e[j], b.e[j], c, 0, 0, 0);
+        return c;
+    }
+};
+template <typename T, int FM>
+__global__ __launch_bounds__(1024) void k_fc_few(FcNtArgs a, int tiles_n) {
+    typedef MmaFew<T> X;
+    constexpr int W = 16;
+    __shared__ float sums[W][FM * 256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
+    const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * (FM * 16);
+    const int n0 = (int)(blockIdx.x % tiles_n) * 16;
+    const float *w = a.W + (size_t)(n0 + lr < a.N ? n0 + lr : a.N - 1) * a.ldw;      // (rows behind the last: any row, their results go nowhere)
+    const T *x[FM];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int64_t m = m0 + j * 16 + lr;
+        x[j] = (const T *)a.A + (m < a.M ? m : a.M - 1) * a.lda;
+    }
+    f32x4 acc[FM];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int full = a.K / X::KS, c = lg * Chunk<T>::N;
+#pragma unroll 4
+    for (int s = wave; s < full; s += W) {
+        Chunk<T> fw, fx;
+        load_w<T>(fw, w, s * X::KS + c, 0x7fffffff);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            fx.u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(x[j] + s * X::KS + c);
+            acc[j] = X::mma(fw, fx, acc[j]);
+        }
+    }
+    if (a.K % X::KS && full % W == wave) {
+        Chunk<T> fw, fx;
+        load_w<T>(fw, w, full * X::KS + c, a.K);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            fx.load(x[j], full * X::KS + c, a.K);
+            acc[j] = X::mma(fw, fx, acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) *reinterpret_cast<f32x4 *>(&sums[wave][(j * 16 + lr) * 16 + lg * 4]) = acc[j];
+    __syncthreads();
+    const int64_t m = m0 + (threadIdx.x >> 4);
+    const int n = n0 + (threadIdx.x & 15);
+    if ((int)threadIdx.x >= FM * 256 || m >= a.M || n >= a.N) return;
+    float v[1] = {0.f};
+#pragma unroll
+    for (int q = 0; q < W; ++q) v[0] += sums[q][threadIdx.x];
+    if (a.bias) v[0] += a.bias[n];
+    if (a.Z) ((T *)a.Z)[m * a.ldz + n] = (T)v[0];
+    act_apply(v, a.act);
+    if (a.R) v[0] += (float)((const T *)a.R)[m * a.ldr + n];
+    ((T *)a.Y)[m * a.ldy + n] = (T)v[0];
 }
 
 // The weights of a product in the activations' type, laid out for k_fc_nt_big: rows padded with zeros to a multiple of BK and of BN
@@ -212,14 +352,6 @@ template <typename T> __global__ __launch_bounds__(256) void k_cast_w(const floa
 
 constexpr int BIG_M = 256, BIG_K = 64, BIG_GROUP = 8;
 typedef __attribute__((address_space(3))) void lds_void;
-// all but the last n loads have landed and every LDS read has returned (the builtin, which the compiler's own wait counting sees: behind
-// waits written in assembly it took an epilogue's loads for still pending and waited for everything inside the product's loop)
-#define PS_WAIT_LOADS(n)                                                        \
-    do {                                                                        \
-        asm volatile("" ::: "memory");                                          \
-        __builtin_amdgcn_s_waitcnt(((n) & 15) | 0x70 | (((n) >> 4) << 14));     \
-        asm volatile("" ::: "memory");                                          \
-    } while (0)
 
 // 16-bit operands, a 256 x BN tile per workgroup of 8 waves, one workgroup a CU.  BN = 256 (waves
 // 2 x 4, 128 x 64 each) asks least of L2 and of LDS per product; BN = 128 (waves 4 x 2, 64 x 64 each) is for outputs of so few tiles
@@ -425,7 +557,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T 
 // 4 rows of a transposing read lie in 4 different bank groups.  The workgroups of the first row of tiles also multiply dz by a
 // fragment of ones: db, row K of the slab.
 template <typename T>
-__global__ __launch_bounds__(256) void k_fc_tn(FcTnArgs a, int tiles_n, int tiles) {
+__global__ __launch_bounds__(256, 2) void k_fc_tn(FcTnArgs a, int tiles_n, int tiles) {
     typedef Mma<T> X;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int CN = Chunk<T>::N, BT = 128, ROWS = F32 ? 32 : 64, PER = BT / CN, P = ROWS * PER / 256, TILE = X::TILE, FK = BT / 2 / TILE, FN = BT / 2 / TILE;
@@ -698,11 +830,11 @@ int grid_ok(int64_t blocks) {
     return blocks * 256 < (1ll << 32) ? PS_OK : ps_set_err(PS_E_UNSUPPORTED, "the batch needs more workgroups than one launch has");
 }
 
-template <typename T, int BM, int BN> int nt_go(const FcNtArgs &a, hipStream_t st) {
+template <typename T, int BM, int BN, int AHEAD> int nt_go(const FcNtArgs &a, hipStream_t st) {
     const int tiles_n = cdiv(a.N, BN);
     const int64_t blocks = (int64_t)tiles_n * cdiv(a.M, BM);
     PSCHK(grid_ok(blocks));
-    hipLaunchKernelGGL((k_fc_nt<T, BM, BN>), dim3((unsigned)blocks), dim3(256), 0, st, a, tiles_n);
+    hipLaunchKernelGGL((k_fc_nt<T, BM, BN, AHEAD>), dim3((unsigned)blocks), dim3(256), 0, st, a, tiles_n);
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
@@ -724,9 +856,26 @@ template <typename T, int BN> int nt_big(const FcNtArgs &a, void *ws, hipStream_
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
+template <typename T, int FM> int few_go(const FcNtArgs &a, hipStream_t st) {
+    const int tiles_n = cdiv(a.N, 16);
+    const int64_t blocks = (int64_t)tiles_n * cdiv(a.M, FM * 16);
+    PSCHK(grid_ok(4 * blocks));
+    hipLaunchKernelGGL((k_fc_few<T, FM>), dim3((unsigned)blocks), dim3(1024), 0, st, a, tiles_n);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
+}
+#ifndef A64
+#define A64 2
+#endif
+#ifndef A128
+#define A128 2
+#endif
 template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
-    if ((int64_t)cdiv(a.M, 128) * cdiv(a.N, 128) >= 256) return nt_go<T, 128, 128>(a, st);
-    return nt_go<T, 64, 64>(a, st);
+    // below one 64 x 64 tile for each CU its chain of staged steps is what a call costs (bf16, 256 x 4096 -> 1024: 59 us, few rows' kernel 21;
+    // f32, 1000 x 275 -> 150: 13 / 6); at one a CU the tiles win (bf16, 1000 x 512 -> 1024: 11 / 16; 4096 x 429 -> 512: 15 / 60)
+    if (a.M <= 64 || (int64_t)cdiv(a.M, 64) * cdiv(a.N, 64) < 256) return a.M <= 16 ? few_go<T, 1>(a, st) : a.M <= 32 ? few_go<T, 2>(a, st) : few_go<T, 4>(a, st);
+    if ((int64_t)cdiv(a.M, 128) * cdiv(a.N, 128) >= 256) return nt_go<T, 128, 128, sizeof(T) == 4 ? A128 : 1>(a, st);
+    return nt_go<T, 64, 64, A64>(a, st);
 }
 template <typename T> int tn_t(const FcTnArgs &a, hipStream_t st) {
     const int tiles_n = cdiv(a.N, 128), tiles = tiles_n * cdiv(a.K, 128);

@@ -65,6 +65,10 @@ typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
 template <int SIZE> struct AtElem { typedef u32x4_at2 v; };
 template <> struct AtElem<4> { typedef u32x4_at4 v; };
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_at2 __attribute__((aligned(2)));
+template <int SIZE> struct AtElem4 { typedef u32x2_at2 v; };      // 4 elements
+template <> struct AtElem4<4> { typedef u32x4_at4 v; };
 
 // 16 bytes of one row in registers: 4 f32 or 8 16-bit values.  A row may start at any multiple of its element's size (odd row strides,
 // views into wider rows): the type's alignment says so and the memory unit takes such a load whole.
@@ -85,6 +89,22 @@ template <typename T> struct Chunk {
                 if (c + N <= n) { *reinterpret_cast<unaligned_t *>(row + c) = u; return; }
 #pragma unroll
         for (int j = 0; j < N; ++j)
+            if (c + j < n) row[c + j] = e[j];
+    }
+};
+// 4 values of one row, at any alignment of theirs
+template <typename T> struct Quad {
+    typedef typename AtElem4<(int)sizeof(T)>::v bits_t;
+    T e[4];
+    __device__ __forceinline__ void load(const T *row, int c, int n) {
+        if (c + 4 <= n) { const bits_t b = *reinterpret_cast<const bits_t *>(row + c); __builtin_memcpy(e, &b, 4 * sizeof(T)); return; }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = c + j < n ? row[c + j] : (T)0.f;
+    }
+    __device__ __forceinline__ void store(T *row, int c, int n) const {
+        if (c + 4 <= n) { bits_t b; __builtin_memcpy(&b, e, 4 * sizeof(T)); *reinterpret_cast<bits_t *>(row + c) = b; return; }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
             if (c + j < n) row[c + j] = e[j];
     }
 };
