@@ -534,63 +534,80 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
     }
 }
 
+// dz = dy act'(z), rounded to the type; z NULL: a copy.  dz's rows are 16-byte pieces, zeros behind the width.
 template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T *dy, int64_t lddy, const T *z, int64_t ldz, T *dz, int64_t lddz, int M, int N, int act) {
-    const int64_t per = (N + Chunk<T>::N - 1) / Chunk<T>::N, total = per * M;
+    const int64_t per = lddz / Chunk<T>::N, total = per * M;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t m = i / per;
         const int c = (int)(i % per) * Chunk<T>::N;
         Chunk<T> d, v;
-        d.load(dy + m * lddy, c, N);
-        v.load(z + m * ldz, c, N);
+        d.zero();
+        if (c < N) {
+            d.load(dy + m * lddy, c, N);
+            if (z) {
+                v.load(z + m * ldz, c, N);
 #pragma unroll
-        for (int j = 0; j < Chunk<T>::N; ++j) {
-            const float zz = (float)v.e[j];
-            d.e[j] = act == PS_ACT_RELU ? (zz > 0.f ? d.e[j] : (T)0.f) : (T)((float)d.e[j] * act_slope(zz, act));
+                for (int j = 0; j < Chunk<T>::N; ++j) {
+                    const float zz = (float)v.e[j];
+                    d.e[j] = act == PS_ACT_RELU ? (zz > 0.f ? d.e[j] : (T)0.f) : (T)((float)d.e[j] * act_slope(zz, act));
+                }
+            }
         }
-        d.store(dz + m * lddz, c, N);
+        *reinterpret_cast<u32x4 *>(dz + m * lddz + c) = d.u;
     }
 }
 
-// One 128 x 128 tile of x^T dz over one part of the batch.  LDS holds the rows as they lie in memory; 16-bit fragments need 8 values
+// One BT x BT tile of x^T dz over one part of the batch.  LDS holds the rows as they lie in memory; 16-bit fragments need 8 values
 // down a column, which the transposing LDS read delivers (16 lanes read 4 rows x 16 columns and get a column's 4 rows each).  The order
-// of the sum inside a step is the same for both operands and otherwise free.  32-byte pieces are exchanged by the row's low bits: the
-// 4 rows of a transposing read lie in 4 different bank groups.  The workgroups of the first row of tiles also multiply dz by a
+// of the sum inside a step is the same for both operands and otherwise free.  32-byte pieces are exchanged by a row key: the 8 rows
+// that 32 lanes of a transposing read touch lie in different banks.  The workgroups of the first row of tiles also multiply dz by a
 // fragment of ones: db, row K of the slab.
-template <typename T>
-__global__ __launch_bounds__(256, 2) void k_fc_tn(FcTnArgs a, int tiles_n, int tiles) {
+// Two steps ahead in registers, as in k_fc_nt: the step that M cuts off goes first, columns behind K and N are read from the row's start
+// (their results go nowhere), and only a tile whose last 16-byte piece the width cuts off (CUT) loads element by element.
+template <typename T, int BT, bool CUT>
+__device__ __forceinline__ void fc_tn_tile(const FcTnArgs &a, int tiles_n, int split, int tile, u32x4 *lds) {
     typedef Mma<T> X;
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int CN = Chunk<T>::N, BT = 128, ROWS = F32 ? 32 : 64, PER = BT / CN, P = ROWS * PER / 256, TILE = X::TILE, FK = BT / 2 / TILE, FN = BT / 2 / TILE;
-    __shared__ u32x4 sX[2][ROWS * PER], sD[2][ROWS * PER];
-    const int id = xcd_tile(blockIdx.x, gridDim.x);
-    const int split = id / tiles, tile = id % tiles, k0 = (tile / tiles_n) * BT, n0 = (tile % tiles_n) * BT;
+    constexpr int CN = Chunk<T>::N, ROWS = F32 ? 32 : 64, PER = BT / CN, P = ROWS * PER / 256, TILE = X::TILE, FK = BT / 2 / TILE, FN = BT / 2 / TILE;
+    constexpr int BUF = ROWS * PER;              // pieces of one operand's step; lds: [step][x | dz]
+    const int k0 = (tile / tiles_n) * BT, n0 = (tile % tiles_n) * BT;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = (wave >> 1) * (BT / 2), wn = (wave & 1) * (BT / 2);
+    auto key = [](int row) { return F32 ? 0 : BT == 128 ? row & 7 : (row >> 1) & 3; };
     // this part's rows: whole steps, dealt evenly
-    const int64_t all = ((int64_t)a.M + ROWS - 1) / ROWS;
-    const int64_t s_lo = all * split / a.nsplit, s_hi = all * (split + 1) / a.nsplit;
-    Chunk<T> rx[P], rd[P];
-    int dst[P];
+    const int64_t all = ((int64_t)a.M + ROWS - 1) / ROWS, s_lo = all * split / a.nsplit, s_hi = all * (split + 1) / a.nsplit;
+    const int cut = s_hi * ROWS > a.M ? 1 : 0, steps = (int)(s_hi - s_lo), full = steps - cut;
+    Chunk<T> rx[2][P], rd[2][P];
+    int dst[P], cx[P], cd[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const int q = tid + i * 256, row = q / PER, c = q % PER;
-        dst[i] = row * PER + (F32 ? c : c ^ ((row & 7) << 1));
+        dst[i] = row * PER + (c ^ (key(row) << 1));
+        cx[i] = k0 + c * CN; cd[i] = n0 + c * CN;
+        if (!CUT) { cx[i] = cx[i] < a.K ? cx[i] : 0; cd[i] = cd[i] < a.N ? cd[i] : 0; }
     }
-    auto fetch = [&](int64_t s) {
+    auto fetch = [&](int set, int64_t step) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int q = tid + i * 256, row = q / PER, c = (q % PER) * CN;
-            const int64_t m = s * ROWS + row;
-            if (m < a.M) {
-                rx[i].load((const T *)a.X + m * a.ldx, k0 + c, a.K);
-                rd[i].load((const T *)a.D + m * a.ldd, n0 + c, a.N);
-            } else {
-                rx[i].zero(); rd[i].zero();
+            const int64_t m = (s_lo + step) * ROWS + (tid + i * 256) / PER;
+            const T *px = (const T *)a.X + m * a.ldx, *pd = (const T *)a.D + m * a.ldd;
+            if constexpr (CUT) { rx[set][i].load(px, cx[i], a.K); rd[set][i].load(pd, cd[i], a.N); }
+            else {
+                rx[set][i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(px + cx[i]);
+                rd[set][i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(pd + cd[i]);
             }
         }
     };
-    auto put = [&](int buf) {
+    auto fetch_cut = [&]() {                     // rows behind the last are zeros
 #pragma unroll
-        for (int i = 0; i < P; ++i) { sX[buf][dst[i]] = rx[i].u; sD[buf][dst[i]] = rd[i].u; }
+        for (int i = 0; i < P; ++i) {
+            const int64_t m = (s_hi - 1) * ROWS + (tid + i * 256) / PER;
+            rx[0][i].zero(); rd[0][i].zero();
+            if (m < a.M) { rx[0][i].load((const T *)a.X + m * a.ldx, cx[i], a.K); rd[0][i].load((const T *)a.D + m * a.ldd, cd[i], a.N); }
+        }
+    };
+    auto put = [&](int set, int buf) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) { lds[buf * 2 * BUF + dst[i]] = rx[set][i].u; lds[(buf * 2 + 1) * BUF + dst[i]] = rd[set][i].u; }
     };
     typename X::acc acc[FK][FN], accb[FN];
     constexpr int AE = (int)(sizeof(accb[0]) / 4);
@@ -607,16 +624,13 @@ __global__ __launch_bounds__(256, 2) void k_fc_tn(FcTnArgs a, int tiles_n, int t
     for (int j = 0; j < CN; ++j) ones[j] = (T)1.f;
     const bool do_bias = k0 == 0 && wk == 0;
     const int lr = lane % TILE, lg = lane / TILE;
-    if (s_lo < s_hi) { fetch(s_lo); put(0); }
-    __syncthreads();
-    for (int64_t s = s_lo; s < s_hi; ++s) {
-        const int buf = (int)(s - s_lo) & 1;
-        if (s + 1 < s_hi) fetch(s + 1);
+    auto multiply = [&](int buf) {
+        const u32x4 *sx = lds + buf * 2 * BUF, *sd = sx + BUF;
 #pragma unroll
         for (int ks = 0; ks < (F32 ? 4 : 2); ++ks) {
             typename X::frag fk[FK], fn[FN];
             if constexpr (F32) {
-                const float *lx = reinterpret_cast<const float *>(sX[buf]), *ld = reinterpret_cast<const float *>(sD[buf]);
+                const float *lx = reinterpret_cast<const float *>(sx), *ld = reinterpret_cast<const float *>(sd);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int row = ks * 8 + e * 2 + lg;
@@ -630,15 +644,14 @@ __global__ __launch_bounds__(256, 2) void k_fc_tn(FcTnArgs a, int tiles_n, int t
                 union { typename X::frag f; s16x4 h[2]; } u;
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const u32x4 *base = w ? sD[buf] : sX[buf];
+                    const short *base = reinterpret_cast<const short *>(w ? sd : sx);
 #pragma unroll
-                    for (int i = 0; i < (FK > FN ? FK : FN); ++i) {
-                        const int col = (w ? wn : wk) + i * 16;                  // 32-byte piece col / 16
+                    for (int i = 0; i < FK; ++i) {
+                        const int piece = ((w ? wn : wk) >> 4) + i;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const int row = ks * 32 + h * 16 + lg * 4 + (lr >> 2);
-                            const short *p = reinterpret_cast<const short *>(base) + row * BT + ((col >> 4) ^ (row & 7)) * 16 + (lr & 3) * 4;
-                            u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
+                            u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(base + row * BT + (piece ^ key(row)) * 16 + (lr & 3) * 4));
                         }
                         if (w) fn[i] = u.f; else fk[i] = u.f;
                     }
@@ -649,16 +662,45 @@ __global__ __launch_bounds__(256, 2) void k_fc_tn(FcTnArgs a, int tiles_n, int t
 #pragma unroll
                 for (int j = 0; j < FN; ++j) acc[i][j] = X::mma(fk[i], fn[j], acc[i][j]);
             if (do_bias) {
+                if constexpr (F32) {             // (f32 matrix instructions are the slow ones: plain adds, a lane's own rows)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) accb[j] = X::mma(ones, fn[j], accb[j]);
+                    for (int j = 0; j < FN; ++j) accb[j][0] += (fn[j][0] + fn[j][1]) + (fn[j][2] + fn[j][3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) accb[j] = X::mma(ones, fn[j], accb[j]);
+                }
             }
         }
-        if (s + 1 < s_hi) put(buf ^ 1);
-        __syncthreads();
+    };
+    if (cut) fetch_cut(); else fetch(0, 0);
+    if (!full) {                                 // (a part has at least one step)
+        put(0, 0);
+        PS_WAIT_LDS(); PS_BARRIER();
+        multiply(0);
+    } else {
+        auto ask = [&](int set, int step) { fetch(set, step < steps ? step - cut : full - 1); };
+        auto half = [&](int s, int p) {
+            ask(p, s + p + 2);
+            multiply(p);
+            put(p ^ 1, p ^ 1);
+            PS_WAIT_LDS(); PS_BARRIER();
+        };
+        ask(1, 1);
+        put(0, 0);
+        PS_WAIT_LDS(); PS_BARRIER();
+        int s = 0;
+        for (; s + 2 <= steps; s += 2) { half(s, 0); half(s, 1); }
+        if (s < steps) half(s, 0);
     }
-    float *part = a.part + (size_t)split * (size_t)(a.K + a.nbias) * a.N;
+    // one part: the result itself
+    float *part = a.nsplit == 1 ? a.dst : a.part + (size_t)split * (size_t)(a.K + a.nbias) * a.N;
+    auto leave = [&](size_t i, float v) {
+        if (a.nsplit == 1) { v /= (float)a.M; if (a.accum) v = part[i] + v; }
+        part[i] = v;
+    };
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
+        if constexpr (F32) accb[j][0] += __shfl_xor(accb[j][0], 32);
         const int n = n0 + wn + j * TILE + lr;
         if (n >= a.N) continue;
 #pragma unroll
@@ -666,10 +708,19 @@ __global__ __launch_bounds__(256, 2) void k_fc_tn(FcTnArgs a, int tiles_n, int t
 #pragma unroll
             for (int e = 0; e < AE; ++e) {
                 const int k = k0 + wk + i * TILE + (e >> 2) * 8 + lg * 4 + (e & 3);
-                if (k < a.K) part[(size_t)k * a.N + n] = acc[i][j][e];
+                if (k < a.K) leave((size_t)k * a.N + n, acc[i][j][e]);
             }
-        if (do_bias && lg == 0) part[(size_t)a.K * a.N + n] = accb[j][0];
+        if (do_bias && lg == 0) leave((size_t)a.K * a.N + n, accb[j][0]);
     }
+}
+template <typename T, int BT>
+__global__ __launch_bounds__(256, BT == 64 ? 3 : 2) void k_fc_tn(FcTnArgs a, int tiles_n, int tiles) {
+    constexpr int CN = Chunk<T>::N;
+    __shared__ u32x4 lds[4 * (sizeof(T) == 4 ? 32 : 64) * BT / CN];
+    const int id = xcd_tile(blockIdx.x, gridDim.x), split = id / tiles, tile = id % tiles;
+    const bool cut = (a.K % CN && (tile / tiles_n + 1) * BT > a.K) || (a.N % CN && (tile % tiles_n + 1) * BT > a.N);
+    if (cut) fc_tn_tile<T, BT, true>(a, tiles_n, split, tile, lds);
+    else fc_tn_tile<T, BT, false>(a, tiles_n, split, tile, lds);
 }
 
 // x^T dz, 16-bit: the same machine as k_fc_nt_big with the batch as the sum's axis, 256 x 256 of dW per workgroup over one part of the
@@ -695,16 +746,16 @@ __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, i
     const int64_t all = ((int64_t)a.M + 63) / 64, s_lo = all * split / a.nsplit, s_hi = all * (split + 1) / a.nsplit;
     const int64_t m_lo = s_lo * 64, m_hi = s_hi * 64 < a.M ? s_hi * 64 : a.M;
     const int steps = (int)(s_hi - s_lo), tail = (int)(m_hi - m_lo) - (steps - 1) * 64;      // rows of the last step
-    const auto rsX = __builtin_amdgcn_make_buffer_rsrc((void *)((const T *)a.X + m_lo * a.ldx), 0, (int)(((m_hi - m_lo - 1) * a.ldx + a.K) * 2), 0x00020000);
-    const auto rsW = __builtin_amdgcn_make_buffer_rsrc((void *)((const T *)a.D + m_lo * a.ldd), 0, (int)(((m_hi - m_lo - 1) * a.ldd + a.N) * 2), 0x00020000);
+    const auto rsX = __builtin_amdgcn_make_buffer_rsrc((void *)((const T *)a.X + m_lo * a.ldx), 0, (int)(((m_hi - m_lo - 1) * a.ldx + a.Kload) * 2), 0x00020000);
+    const auto rsW = __builtin_amdgcn_make_buffer_rsrc((void *)((const T *)a.D + m_lo * a.ldd), 0, (int)(((m_hi - m_lo - 1) * a.ldd + a.Nload) * 2), 0x00020000);
     // piece tid of the first 32 rows of a quarter and of the second: row tid / 16 (+ 32), its 16 bytes exchanged within the row
     const int row = tid >> 4, col = ((((tid & 15) >> 1) ^ (row & 7)) * 2 + (tid & 1)) * 8;
     constexpr int OUT = 0x7ffffff0;
     int vx[2], vw[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        vx[h] = k0 + h * 128 + col < a.K ? (int)(row * a.ldx + k0 + h * 128 + col) * 2 : OUT;
-        vw[h] = n0 + h * 128 + col < a.N ? (int)(row * a.ldd + n0 + h * 128 + col) * 2 : OUT;
+        vx[h] = k0 + h * 128 + col < a.Kload ? (int)(row * a.ldx + k0 + h * 128 + col) * 2 : OUT;
+        vw[h] = n0 + h * 128 + col < a.Nload ? (int)(row * a.ldd + n0 + h * 128 + col) * 2 : OUT;
     }
     const int sx = (int)a.ldx * 64, sw = (int)a.ldd * 64;                    // bytes of 32 rows
     auto ask = [&](int t, const __amdgpu_buffer_rsrc_t &rs, int v, int s32, int at) {
@@ -806,24 +857,75 @@ __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, i
     for (int i = 0; i < 4; ++i) {
         const int n = n0 + (i >> 1) * 128 + wn * 32 + (i & 1) * 16 + lg * 4;
         if (n >= a.N) continue;
+        auto row = [&](int k, const f32x4 &v) {
+            Quad<float> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.e[e] = v[e];
+            o.store(part + (size_t)k * a.N, n, a.N);
+        };
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int k = k0 + (j >> 2) * 128 + wm * 64 + (j & 3) * 16 + lr;
-            if (k < a.K) *reinterpret_cast<f32x4 *>(part + (size_t)k * a.N + n) = acc[i][j];
+            if (k < a.K) row(k, acc[i][j]);
         }
-        if (lr == 0) *reinterpret_cast<f32x4 *>(part + (size_t)(a.K + kt * 2 + wm) * a.N + n) = accb[i];
+        if (lr == 0) row(a.K + kt * 2 + wm, accb[i]);
     }
 }
 
-__global__ __launch_bounds__(256) void k_fc_grad_reduce(FcTnArgs a, float *__restrict__ dst, int accum) {
-    const int64_t n = (int64_t)a.K * a.N, i = (int64_t)blockIdx.x * 256 + threadIdx.x, slab = (int64_t)(a.K + a.nbias) * a.N;
-    if (i >= n + a.N) return;
-    const int rows = i < n ? 1 : a.nbias;
+// The slabs' sum and mean: dW over the parts, db over the parts and their rows.  A wave takes 256 neighbouring elements (4 a lane) and 8
+// slabs at a time.  W = 1: every wave its own elements; W = 16, many slabs: the waves of a workgroup share them out and are added in
+// wave order.  The workgroups behind dW's do db, 64 columns each.
+template <int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 1024) void k_fc_grad_reduce(FcTnArgs a, int dw_blocks) {
+    typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
+    __shared__ f32x4 sums[W == 1 ? 4 : 16][64];
+    const int64_t n = (int64_t)a.K * a.N, slab = (int64_t)(a.K + a.nbias) * a.N;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int WAVES = W == 1 ? 4 : 16;
+    auto finish = [&](int64_t i, float s) { s /= (float)a.M; a.dst[i] = a.accum ? a.dst[i] + s : s; };
+    if ((int)blockIdx.x < dw_blocks) {
+        const int64_t i = (W == 1 ? ((int64_t)blockIdx.x * 4 + wave) : (int64_t)blockIdx.x) * 256 + lane * 4;
+        const int64_t ic = i + 4 <= n ? i : n >= 4 ? n - 4 : 0;              // (n < 4: the elements behind dW are db's, in bounds)
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int z0 = W == 1 ? 0 : wave; z0 < a.nsplit; z0 += 8 * W) {
+            f32x4 v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const f32x4_at4 *>(a.part + (z0 + q * W < a.nsplit ? z0 + q * W : a.nsplit - 1) * slab + ic);
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (z0 + q * W < a.nsplit) s += v[q];
+        }
+        if constexpr (W > 1) {
+            sums[wave][lane] = s;
+            __syncthreads();
+            if (wave) return;
+#pragma unroll
+            for (int w = 1; w < W; ++w) s += sums[w][lane];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)              // (a lane at dW's end read from n - 4 on and keeps what is its own)
+            if (ic + e >= i && ic + e < n) finish(ic + e, s[e]);
+        return;
+    }
+    const int col = ((int)blockIdx.x - dw_blocks) * 64 + lane, cc = col < a.N ? col : a.N - 1, rows = a.nsplit * a.nbias;
     float s = 0.f;
-    for (int z = 0; z < a.nsplit; ++z)
-        for (int r = 0; r < rows; ++r) s += a.part[z * slab + i + (int64_t)r * a.N];
-    s /= (float)a.M;
-    dst[i] = accum ? dst[i] + s : s;
+    for (int z0 = wave; z0 < rows; z0 += 8 * WAVES) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int z = z0 + q * WAVES < rows ? z0 + q * WAVES : rows - 1;
+            v[q] = a.part[(z / a.nbias) * slab + n + (int64_t)(z % a.nbias) * a.N + cc];
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (z0 + q * WAVES < rows) s += v[q];
+    }
+    sums[wave][lane][0] = s;
+    __syncthreads();
+    if (wave || col >= a.N) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) s += sums[w][lane][0];
+    finish(n + col, s);
 }
 
 int grid_ok(int64_t blocks) {
@@ -838,20 +940,39 @@ template <typename T, int BM, int BN, int AHEAD> int nt_go(const FcNtArgs &a, hi
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
-// Which tile of k_fc_nt_big a product takes, 0: none.  Its loads want 16-byte pieces and its offsets 31 bits; 128 columns cost 0.6 of
-// 256 (measured on full chips), so they win where they halve the rounds of the 256 CUs; below half a round the small tiles win.
-int big_tile(int type, const FcNtArgs &a) {
-    if (type == PS_T_F32 || (uintptr_t)a.A % 16 || a.lda % 8 || a.lda > (1 << 21) || a.K > (1 << 21)) return 0;
-    const int64_t tm = cdiv(a.M, BIG_M), t2 = tm * cdiv(a.N, 256), t1 = tm * cdiv(a.N, 128);
-    if (t1 < 128 || t1 >= (1 << 30)) return 0;
-    return 10 * cdiv(t2, 256) <= 6 * cdiv(t1, 256) ? 256 : 128;
+template <typename T>
+int ag_t(int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st) {
+    const int64_t blocks = (lddz / Chunk<T>::N * M + 255) / 256;
+    hipLaunchKernelGGL((k_act_grad<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, (const T *)dy, lddy, (const T *)z, ldz,
+                       (T *)dz, lddz, M, N, act);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
 }
-template <typename T, int BN> int nt_big(const FcNtArgs &a, void *ws, hipStream_t st) {
+// Whether and how a product takes k_fc_nt_big.  Its loads want 16-byte pieces and its offsets 31 bits; rows that start elsewhere are
+// copied first, which a product of 256 columns or more pays for (bf16, 20000 x 1001 -> 1001 relu: 118 us without, 79 with).
+// 128 columns cost 0.6 of 256 (measured on full chips), so they win where they halve the rounds of the 256 CUs; below half a round the
+// small tiles win.
+struct NtPlan { int bn = 0; bool pack = false; };
+NtPlan nt_plan(int type, const FcNtArgs &a) {
+    NtPlan p;
+    if (type == PS_T_F32 || a.K > (1 << 21)) return p;
+    p.pack = (uintptr_t)a.A % 16 || a.lda % 8 || a.lda > (1 << 21);
+    const int64_t tm = cdiv(a.M, BIG_M), t2 = tm * cdiv(a.N, 256), t1 = tm * cdiv(a.N, 128);
+    if (t1 < 128 || t1 >= (1 << 30) || (p.pack && a.N < 256)) return p;
+    p.bn = 10 * cdiv(t2, 256) <= 6 * cdiv(t1, 256) ? 256 : 128;
+    return p;
+}
+template <typename T, int BN> int nt_big(FcNtArgs a, bool pack, char *ws, hipStream_t st) {
     const int Kp = (int)round_up(a.K, BIG_K), Np = (int)round_up(a.N, BN), tiles_n = Np / BN, tiles_m = cdiv(a.M, BIG_M);
     const int64_t pieces = (int64_t)Kp / 8 * Np;
     PSCHK(grid_ok(cdiv(pieces, 256)));
-    hipLaunchKernelGGL((k_cast_w<T>), dim3((unsigned)cdiv(pieces, 256)), dim3(256), 0, st, a.W, a.ldw, a.N, a.K, (T *)ws, Kp, Np);
     PSCHK(grid_ok(2ll * tiles_m * tiles_n));
+    hipLaunchKernelGGL((k_cast_w<T>), dim3((unsigned)cdiv(pieces, 256)), dim3(256), 0, st, a.W, a.ldw, a.N, a.K, (T *)ws, Kp, Np);
+    if (pack) {
+        char *x = ws + round_up((int64_t)Kp * Np * 2, 256);
+        PSCHK((ag_t<T>(PS_ACT_NONE, a.A, a.lda, nullptr, 0, x, Kp, a.M, a.K, st)));
+        a.A = x; a.lda = a.K = Kp;
+    }
     hipLaunchKernelGGL((k_fc_nt_big<T, BN>), dim3((unsigned)(tiles_m * tiles_n)), dim3(512), 0, st, a, (const T *)ws, Kp, tiles_m, tiles_n);
     HIPCHK(hipGetLastError());
     return PS_OK;
@@ -877,14 +998,15 @@ template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
     if ((int64_t)cdiv(a.M, 128) * cdiv(a.N, 128) >= 256) return nt_go<T, 128, 128, sizeof(T) == 4 ? A128 : 1>(a, st);
     return nt_go<T, 64, 64, A64>(a, st);
 }
-template <typename T> int tn_t(const FcTnArgs &a, hipStream_t st) {
-    const int tiles_n = cdiv(a.N, 128), tiles = tiles_n * cdiv(a.K, 128);
+template <typename T, int BT> int tn_go(const FcTnArgs &a, hipStream_t st) {
+    const int tiles_n = cdiv(a.N, BT), tiles = tiles_n * cdiv(a.K, BT);
     const int64_t blocks = (int64_t)tiles * a.nsplit;
     PSCHK(grid_ok(blocks));
-    hipLaunchKernelGGL((k_fc_tn<T>), dim3((unsigned)blocks), dim3(256), 0, st, a, tiles_n, tiles);
+    hipLaunchKernelGGL((k_fc_tn<T, BT>), dim3((unsigned)blocks), dim3(256), 0, st, a, tiles_n, tiles);
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
+template <typename T> int tn_t(const FcTnArgs &a, hipStream_t st) { return a.tile == 128 ? tn_go<T, 128>(a, st) : tn_go<T, 64>(a, st); }
 template <typename T> int tn_big(const FcTnArgs &a, hipStream_t st) {
     const int tiles_n = cdiv(a.N, 256), tiles_k = cdiv(a.K, 256);
     const int64_t blocks = (int64_t)tiles_n * tiles_k * a.nsplit;
@@ -893,25 +1015,18 @@ template <typename T> int tn_big(const FcTnArgs &a, hipStream_t st) {
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
-template <typename T>
-int ag_t(int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st) {
-    const int64_t blocks = ((int64_t)cdiv(N, Chunk<T>::N) * M + 255) / 256;
-    hipLaunchKernelGGL((k_act_grad<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, (const T *)dy, lddy, (const T *)z, ldz,
-                       (T *)dz, lddz, M, N, act);
-    HIPCHK(hipGetLastError());
-    return PS_OK;
-}
-
 }  // namespace
 
 size_t fc_nt_workspace(int type, const FcNtArgs &a) {
-    const int bn = big_tile(type, a);
-    return bn ? (size_t)round_up(a.K, BIG_K) * (size_t)round_up(a.N, bn) * 2 : 0;
+    const NtPlan p = nt_plan(type, a);
+    if (!p.bn) return 0;
+    const int64_t Kp = round_up(a.K, BIG_K), w = round_up(Kp * round_up(a.N, p.bn) * 2, 256);
+    return (size_t)(w + (p.pack ? Kp * a.M * 2 : 0));
 }
-int launch_fc_nt(int type, const FcNtArgs &a, void *ws, hipStream_t st) {
-    const int bn = big_tile(type, a);
-    if (bn == 256) return type == PS_T_BF16 ? nt_big<__bf16, 256>(a, ws, st) : nt_big<_Float16, 256>(a, ws, st);
-    if (bn == 128) return type == PS_T_BF16 ? nt_big<__bf16, 128>(a, ws, st) : nt_big<_Float16, 128>(a, ws, st);
+int launch_fc_nt(int type, const FcNtArgs &a, char *ws, hipStream_t st) {
+    const NtPlan p = nt_plan(type, a);
+    if (p.bn == 256) return type == PS_T_BF16 ? nt_big<__bf16, 256>(a, p.pack, ws, st) : nt_big<_Float16, 256>(a, p.pack, ws, st);
+    if (p.bn == 128) return type == PS_T_BF16 ? nt_big<__bf16, 128>(a, p.pack, ws, st) : nt_big<_Float16, 128>(a, p.pack, ws, st);
     return type == PS_T_F32 ? nt_t<float>(a, st) : type == PS_T_BF16 ? nt_t<__bf16>(a, st) : nt_t<_Float16>(a, st);
 }
 int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st) {
@@ -919,32 +1034,49 @@ int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void 
            : type == PS_T_BF16 ? ag_t<__bf16>(act, dy, lddy, z, ldz, dz, lddz, M, N, st)
                                : ag_t<_Float16>(act, dy, lddy, z, ldz, dz, lddz, M, N, st);
 }
-// How dW is taken apart: a.big, a.nsplit, a.nbias.  The large tiles want 16-byte pieces, offsets of 31 bits inside a part, and parts of at
-// least 16 steps; one workgroup for each of the 256 CUs.
+// How dW is taken apart: a.tile, a.nsplit, a.nbias, and what has to be copied into 16-byte pieces first (pack_x, pack_d: the caller lays
+// rows of 8-element multiples out and tells where).  The 256 tiles: such pieces, offsets of 31 bits inside a part, parts of at least 16
+// steps, one workgroup for each of the 256 CUs; a copy is paid for from 256 columns of the other operand on.  The smaller ones: two
+// workgroups a CU, no part shorter than four steps, and 128 only where parts stay eight steps long -- shorter ones are all start and end
+// (bf16, 4096 x 429 -> 512: 34 us in parts of 4 steps of 128, 24 by 64; 16384 x 1001 -> 1001 in parts of 32: 159 / 343).
 void fc_tn_plan(int type, FcTnArgs &a) {
     const bool f32 = type == PS_T_F32;
     const int64_t big = (int64_t)cdiv(a.N, 256) * cdiv(a.K, 256), steps = cdiv(a.M, 64);
-    a.big = 0;
-    if (!f32 && !((uintptr_t)a.X % 16 || (uintptr_t)a.D % 16 || a.ldx % 8 || a.ldd % 8 || a.K % 8 || a.N % 8) && big * steps >= 2048) {
+    a.pack_x = (uintptr_t)a.X % 16 || a.ldx % 8 || a.K % 8;
+    a.pack_d = (uintptr_t)a.D % 16 || a.ldd % 8 || (a.D && a.N % 8);         // (D NULL: dz, which will lie in pieces in any case)
+    a.Kload = (int)round_up(a.K, 8); a.Nload = (int)round_up(a.N, 8);
+    if (!f32 && big * steps >= 2048 && !(a.pack_x && a.N < 256) && !(a.pack_d && a.K < 256)) {
         int64_t s = big >= 256 ? 1 : 256 / big;
         if (s > steps / 16) s = steps / 16 > 0 ? steps / 16 : 1;
-        const int64_t rows = (cdiv(steps, s) + 1) * 64, ld = a.ldx > a.ldd ? a.ldx : a.ldd;
-        if (rows * ld * 2 < (1ll << 31) - 64) { a.big = 1; a.nsplit = (int)s; a.nbias = 2 * cdiv(a.K, 256); return; }
+        const int64_t lx = a.pack_x ? a.Kload : a.ldx, ld = a.pack_d ? a.Nload : a.ldd;
+        if ((cdiv(steps, s) + 1) * 64 * (lx > ld ? lx : ld) * 2 < (1ll << 31) - 64) { a.tile = 256; a.nsplit = (int)s; a.nbias = 2 * cdiv(a.K, 256); return; }
     }
-    const int64_t tiles = (int64_t)cdiv(a.N, 128) * cdiv(a.K, 128), st = cdiv(a.M, f32 ? 32 : 64);
-    int64_t s = (512 + tiles - 1) / tiles;               // two workgroups for each of the 256 CUs
-    if (s > st / 4) s = st / 4;                          // and no part shorter than four steps
-    a.nsplit = (int)(s < 1 ? 1 : s); a.nbias = 1;
+    a.pack_x = a.pack_d = 0;
+    const int64_t st = cdiv(a.M, f32 ? 32 : 64);
+    a.nbias = 1;
+    for (a.tile = 128;; a.tile = 64) {
+        const int64_t tiles = (int64_t)cdiv(a.N, a.tile) * cdiv(a.K, a.tile);
+        int64_t s = (512 + tiles - 1) / tiles;
+        if (s > st / 4) s = st / 4;
+        a.nsplit = (int)(s < 1 ? 1 : s);
+        if (a.tile == 64 || st >= 8 * a.nsplit) return;
+    }
 }
 int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st) {
-    if (a.big) return type == PS_T_BF16 ? tn_big<__bf16>(a, st) : tn_big<_Float16>(a, st);
-    return type == PS_T_F32 ? tn_t<float>(a, st) : type == PS_T_BF16 ? tn_t<__bf16>(a, st) : tn_t<_Float16>(a, st);
-}
-// The slabs' sum and mean: dW's rows over the parts, db's over the parts and their rows 
-int launch_fc_grad_reduce(const FcTnArgs &a, float *dst, int accum, hipStream_t st) {
-    const int64_t n = (int64_t)(a.K + 1) * a.N;
-    PSCHK(grid_ok((n + 255) / 256));
-    hipLaunchKernelGGL(k_fc_grad_reduce, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, dst, accum);
+    if (a.tile == 256) PSCHK(type == PS_T_BF16 ? tn_big<__bf16>(a, st) : tn_big<_Float16>(a, st));
+    else PSCHK(type == PS_T_F32 ? tn_t<float>(a, st) : type == PS_T_BF16 ? tn_t<__bf16>(a, st) : tn_t<_Float16>(a, st));
+    if (a.nsplit * a.nbias == 1) return PS_OK;               // (the kernel has left the result itself)
+    const int64_t n = (int64_t)a.K * a.N;
+    const int db = cdiv(a.N, 64);
+    if (a.nsplit >= 16) {
+        const int64_t dw = (n + 255) / 256;
+        PSCHK(grid_ok(4 * (dw + db)));
+        hipLaunchKernelGGL(k_fc_grad_reduce<16>, dim3((unsigned)(dw + db)), dim3(1024), 0, st, a, (int)dw);
+    } else {
+        const int64_t dw = (n + 1023) / 1024;
+        PSCHK(grid_ok(dw + db));
+        hipLaunchKernelGGL(k_fc_grad_reduce<1>, dim3((unsigned)(dw + db)), dim3(256), 0, st, a, (int)dw);
+    }
     HIPCHK(hipGetLastError());
     return PS_OK;
 }

@@ -37,21 +37,23 @@ struct FcNtArgs {
     void *Y; int64_t ldy;
     int M, N, K, act;
 };
-size_t fc_nt_workspace(int type, const FcNtArgs &a);                        // bytes of ws that launch_fc_nt needs, 16-byte aligned
-int launch_fc_nt(int type, const FcNtArgs &a, void *ws, hipStream_t st);
-// dz = dy * act'(z), rounded to the type; rows of lddz elements
+size_t fc_nt_workspace(int type, const FcNtArgs &a);                        // bytes of ws that launch_fc_nt needs, 256-byte aligned
+int launch_fc_nt(int type, const FcNtArgs &a, char *ws, hipStream_t st);
+// dz = dy * act'(z), rounded to the type (act NONE: a copy); rows of lddz elements, a multiple of 8, 16-byte aligned, zeros behind N
 int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz, int M, int N, hipStream_t st);
-// part[s][k][n] = sum over the s-th part of m of X[m][k] * D[m][n], k < K; the nbias rows behind: shares of the sum of D[m][n]
+// dst[k][n] = (accum ? dst[k][n] : 0) + (sum over m of X[m][k] * D[m][n]) / M, k < K; row K: of D[m][n].  Through slabs of parts of m,
+// part[nsplit][K + nbias][N], the nbias rows behind: shares of the sum of D[m][n].
 struct FcTnArgs {
     const void *X; int64_t ldx;
-    const void *D; int64_t ldd;
-    float *part;                       // [nsplit][K + nbias][N]
+    const void *D; int64_t ldd;        // D NULL before the plan: rows in 16-byte pieces, ldd a multiple of 8, zeros behind N
     int M, K, N;
-    int big, nsplit, nbias;            // filled by fc_tn_plan
+    int tile, nsplit, nbias;           // filled by fc_tn_plan, and ...
+    int pack_x, pack_d, Kload, Nload;  // ... X / D have to be replaced by a copy in rows of Kload / Nload elements (launch_act_grad, act NONE)
+    float *part, *dst;
+    int accum;
 };
 void fc_tn_plan(int type, FcTnArgs &a);
 int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st);
-int launch_fc_grad_reduce(const FcTnArgs &a, float *dst, int accum, hipStream_t st);      // [K + 1][N]: means over M
 
 #ifdef __HIPCC__
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));

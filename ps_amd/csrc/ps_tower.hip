@@ -236,26 +236,32 @@ extern "C" int ps_fc_res_backward(ps_store_t *s, int layer, int type, int act, c
     float *dst;
     int accum;
     PSCHK(grad_target(s, *p, grad_dev, &dst, &accum));
-    // workspace: [slabs of dW | db][dz][what the product for dx needs]
-    const int64_t lddz = round_up(N, 8);
     FcTnArgs t;
-    t.X = x_dev; t.ldx = ldx; t.D = z_dev ? nullptr : dy_dev; t.ldd = z_dev ? lddz : lddy; t.M = B; t.K = K; t.N = N;      // (dz: 256-byte aligned in the workspace)
+    t.X = x_dev; t.ldx = ldx; t.D = z_dev ? nullptr : dy_dev; t.ldd = z_dev ? round_up(N, 8) : lddy; t.M = B; t.K = K; t.N = N;
+    t.dst = dst; t.accum = accum;
     fc_tn_plan(type, t);
-    const size_t slabs = (size_t)round_up((int64_t)sizeof(float) * (K + t.nbias) * N * t.nsplit, 256), dzs = z_dev ? (size_t)round_up(es * lddz * B, 256) : 0;
     FcNtArgs a;
-    a.A = dy_dev; a.lda = lddy; a.W = p->W; a.ldw = p->ldw; a.bias = nullptr; a.R = skip_dev; a.ldr = skip_dev ? ldskip : 0; a.Z = nullptr; a.ldz = 0;
+    a.A = t.D; a.lda = t.ldd; a.W = p->W; a.ldw = p->ldw; a.bias = nullptr; a.R = skip_dev; a.ldr = skip_dev ? ldskip : 0; a.Z = nullptr; a.ldz = 0;
     a.Y = dx_dev; a.ldy = lddx; a.M = B; a.N = K; a.K = N; a.act = PS_ACT_NONE;
-    if (z_dev) { a.A = nullptr; a.lda = lddz; }
-    char *ws;
-    PSCHK(workspace(s, slabs + dzs + (dx_dev ? fc_nt_workspace(type, a) : 0), &ws));
+    const bool own_dz = z_dev || t.pack_d;       // dz in the workspace: behind an activation, or dy's copy in 16-byte pieces
+    if (own_dz) { t.D = a.A = nullptr; t.ldd = a.lda = round_up(N, 8); }
+    // workspace: [slabs of dW | db][dz][x in pieces][what the product for dx needs], each 256-byte aligned
+    const size_t slabs = t.nsplit * t.nbias == 1 ? 0 : (size_t)round_up((int64_t)sizeof(float) * (K + t.nbias) * N * t.nsplit, 256);
+    const size_t dzs = own_dz ? (size_t)round_up(es * t.ldd * B, 256) : 0, xs = t.pack_x ? (size_t)round_up((int64_t)es * t.Kload * B, 256) : 0;
+    const size_t need = slabs + dzs + xs + (dx_dev ? fc_nt_workspace(type, a) : 0);
+    char *ws = nullptr;
+    if (need) PSCHK(workspace(s, need, &ws));
     t.part = (float *)ws;
-    if (z_dev) {
+    if (own_dz) {
         t.D = a.A = ws + slabs;
-        PSCHK(launch_act_grad(type, act, dy_dev, lddy, z_dev, ldz, ws + slabs, lddz, B, N, st));
+        PSCHK(launch_act_grad(type, act, dy_dev, lddy, z_dev, ldz, ws + slabs, t.ldd, B, N, st));
     }
-    if (dx_dev) PSCHK(launch_fc_nt(type, a, ws + slabs + dzs, st));
+    if (dx_dev) PSCHK(launch_fc_nt(type, a, ws + slabs + dzs + xs, st));
+    if (t.pack_x) {
+        PSCHK(launch_act_grad(type, PS_ACT_NONE, x_dev, ldx, nullptr, 0, ws + slabs + dzs, t.Kload, B, K, st));
+        t.X = ws + slabs + dzs; t.ldx = t.Kload;
+    }
     PSCHK(launch_fc_tn(type, t, st));
-    PSCHK(launch_fc_grad_reduce(t, dst, accum, st));
     if (!grad_dev) p->pending_cnt++;
     return PS_OK;
 }
