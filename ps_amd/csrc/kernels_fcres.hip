@@ -723,6 +723,13 @@ __global__ __launch_bounds__(256, BT == 64 ? 3 : 2) void k_fc_tn(FcTnArgs a, int
     else fc_tn_tile<T, BT, false>(a, tiles_n, split, tile, lds);
 }
 
+// The transposing LDS read.  As a function of a restrict pointer: the compiler then knows what it reads, and does not wait for every load
+// on its way into LDS in front of it (which made every phase of k_fc_tn_big a round trip to memory).
+__device__ __forceinline__ s16x4 read_transposed(const short *__restrict__ p) {
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
+}
+
 // x^T dz, 16-bit: the same machine as k_fc_nt_big with the batch as the sum's axis, 256 x 256 of dW per workgroup over one part of the
 // batch.  A step is 64 rows of both operands; a quarter holds their columns 128 h .. 128 h + 127, so its rows are 256 contiguous bytes.
 // Fragments need 8 values down a column: two transposing LDS reads (16 lanes read 4 rows x 16 columns and get a column's 4 rows each;
@@ -735,14 +742,14 @@ template <typename T>
 __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, int tiles_n) {
     typedef Mma<T> X;
     typedef typename X::frag frag;
-    typedef __attribute__((address_space(3))) s16x4 lds4;
     constexpr int Q = 64 * 16;
     constexpr int OX[2] = {0, 3 * Q}, OW[2] = {Q, 2 * Q};
     __shared__ u32x4 lds[2][4 * Q];              // [step][x0 | w0 | w1 | x1] (w: dz)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
     const bool second = wave >= 4;
     const int tiles = tiles_k * tiles_n, id = xcd_tile(blockIdx.x, gridDim.x), split = id / tiles, tile = id % tiles;
-    const int kt = tile / tiles_n, k0 = kt * 256, n0 = (tile % tiles_n) * 256;
+    // (the shorter side first: what an XCD runs at one time is nearer a square and shares more of both operands in its L2)
+    const int kt = tiles_k < tiles_n ? tile % tiles_k : tile / tiles_n, k0 = kt * 256, n0 = (tiles_k < tiles_n ? tile / tiles_k : tile % tiles_n) * 256;
     const int64_t all = ((int64_t)a.M + 63) / 64, s_lo = all * split / a.nsplit, s_hi = all * (split + 1) / a.nsplit;
     const int64_t m_lo = s_lo * 64, m_hi = s_hi * 64 < a.M ? s_hi * 64 : a.M;
     const int steps = (int)(s_hi - s_lo), tail = (int)(m_hi - m_lo) - (steps - 1) * 64;      // rows of the last step
@@ -780,13 +787,13 @@ __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, i
     for (int j = 0; j < 4; ++j) ox[j] = lo + ((wm * 4 + j) ^ key) * 16;
 #pragma unroll
     for (int i = 0; i < 2; ++i) ow[i] = lo + ((wn * 2 + i) ^ key) * 16;
-    frag fx[2][4], fw[2][4], ones;
+    frag fx[2][4], fw[2][4], fv[2][2], ones;     // [half step][fragment]; fv: the next step's w0, read ahead of its step
 #pragma unroll
     for (int e = 0; e < 8; ++e) ones[e] = (T)1.f;
     auto column = [&](const short *base, int k) {
         union { frag f; s16x4 h[2]; } u;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(base + (k * 32 + h * 16) * 128));
+        for (int h = 0; h < 2; ++h) u.h[h] = read_transposed(base + (k * 32 + h * 16) * 128);
         return u.f;
     };
     auto read_x = [&](int t, int half) {
@@ -795,11 +802,23 @@ __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, i
 #pragma unroll
             for (int j = 0; j < 4; ++j) fx[k][j] = column((const short *)&lds[t & 1][OX[half]] + ox[j], k);
     };
-    auto read_w = [&](int t, int half) {
+    auto read_w1 = [&](int t) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) fw[k][half * 2 + i] = column((const short *)&lds[t & 1][OW[half]] + ow[i], k);
+            for (int i = 0; i < 2; ++i) fw[k][2 + i] = column((const short *)&lds[t & 1][OW[1]] + ow[i], k);
+    };
+    auto read_w0 = [&](int t) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) fv[k][i] = column((const short *)&lds[t & 1][OW[0]] + ow[i], k);
+    };
+    auto take_w0 = [&]() {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) fw[k][i] = fv[k][i];
     };
     auto multiply = [&](int hx, int hw) {
         __builtin_amdgcn_s_setprio(1);
@@ -821,35 +840,39 @@ __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, i
             for (int i = 0; i < 2; ++i) accb[hw * 2 + i] = X::mma(fw[k][hw * 2 + i], ones, accb[hw * 2 + i]);
         if (hw == 1) next_b += 2 * tiles_k;
     };
-    ask_x(0, 0); ask_w(0, 0); ask_w(0, 1); ask_x(0, 1);
+    // The transposing reads are twice as many as k_fc_nt_big's plain ones, and a phase should not hold more of them than the other waves'
+    // matrix instructions cover: w0 is read in the phase before its step (16, 8, 16, 8 reads a phase instead of 24, 8, 16, 0).
+    ask_w(0, 0); ask_x(0, 0); ask_w(0, 1); ask_x(0, 1);
     if (steps > 1) {
-        ask_x(1, 0); ask_w(1, 0); ask_w(1, 1);
+        ask_w(1, 0); ask_x(1, 0); ask_w(1, 1);
         PS_WAIT_LOADS(10);
     } else {
         PS_WAIT_LOADS(0);
     }
     turn();
     if (second) turn();
+    read_w0(0);
     int t = 0;
     for (; t < steps - 2; ++t) {
-        read_x(t, 0); read_w(t, 0); ask_x(t + 1, 1);
-        PS_WAIT_LOADS(10); turn(); multiply(0, 0); add_up(t, 0); turn();
-        read_w(t, 1); ask_x(t + 2, 0);
+        read_x(t, 0); ask_x(t + 1, 1);
+        PS_WAIT_LOADS(10); turn(); take_w0(); multiply(0, 0); add_up(t, 0); turn();
+        read_w1(t); ask_w(t + 2, 0);
         PS_WAIT_LOADS(10); turn(); multiply(0, 1); add_up(t, 1); turn();
-        read_x(t, 1); ask_w(t + 2, 0);
+        read_x(t, 1); ask_x(t + 2, 0);
         PS_WAIT_LOADS(10); turn(); multiply(1, 1); turn();
-        ask_w(t + 2, 1);
+        read_w0(t + 1); ask_w(t + 2, 1);
         PS_WAIT_LOADS(10); turn(); multiply(1, 0); turn();
     }
     for (; t < steps; ++t) {
-        read_x(t, 0); read_w(t, 0);
+        read_x(t, 0);
         if (t + 1 < steps) ask_x(t + 1, 1);
-        PS_WAIT_LOADS(0); turn(); multiply(0, 0); add_up(t, 0); turn();
-        read_w(t, 1);
+        PS_WAIT_LOADS(0); turn(); take_w0(); multiply(0, 0); add_up(t, 0); turn();
+        read_w1(t);
         PS_WAIT_LOADS(0); turn(); multiply(0, 1); add_up(t, 1); turn();
         read_x(t, 1);
         PS_WAIT_LOADS(0); turn(); multiply(1, 1); turn();
-        turn(); multiply(1, 0); turn();
+        if (t + 1 < steps) read_w0(t + 1);
+        PS_WAIT_LOADS(0); turn(); multiply(1, 0); turn();
     }
     if (!second) turn();
     float *part = a.part + (size_t)split * (size_t)(a.K + a.nbias) * a.N;
@@ -1068,7 +1091,7 @@ int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st) {
     if (a.nsplit * a.nbias == 1) return PS_OK;               // (the kernel has left the result itself)
     const int64_t n = (int64_t)a.K * a.N;
     const int db = cdiv(a.N, 64);
-    if (a.nsplit >= 16) {
+    if (a.nsplit >= 16 && n < 256 * 1024) {                  // (from one workgroup of four waves for each CU on they need not share)
         const int64_t dw = (n + 255) / 256;
         PSCHK(grid_ok(4 * (dw + db)));
         hipLaunchKernelGGL(k_fc_grad_reduce<16>, dim3((unsigned)(dw + db)), dim3(1024), 0, st, a, (int)dw);
