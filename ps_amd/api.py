@@ -506,20 +506,19 @@ _TYPES = {}          # a tensor's dtype -> PS_T_*
 
 def _mat(t, name, B=None, width=None, like=None):
     """(pointer, row stride) of a [B][width] device tensor (torch's, or anything with its attributes): checked, never copied."""
-    if t.dim() != 2 or (width is not None and t.shape[1] != width) or (B is not None and t.shape[0] != B):
-        raise N.PsError(N.PS_E_BAD_ARG, "%s: shape %s, wanted [%s][%s]" % (name, tuple(t.shape), "B" if B is None else B, width))
-    ld, inner = t.stride()
-    if inner != 1 and t.shape[1] > 1:
-        raise N.PsError(N.PS_E_BAD_ARG, "%s: the columns of a row must be neighbours (stride %d)" % (name, inner))
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    shape = t.shape
+    if len(shape) != 2 or (width is not None and shape[1] != width) or (B is not None and shape[0] != B):
+        raise N.PsError(N.PS_E_BAD_ARG, "%s: shape %s, wanted [%s][%s]" % (name, tuple(shape), "B" if B is None else B, width))
+    if like is not None and (t.dtype is not like.dtype or t.get_device() != like.get_device()):
         raise N.PsError(N.PS_E_BAD_ARG, "%s: %s on %s, wanted %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
-    if t.shape[0] <= 1:
-        ld = t.shape[1]                                # one row: its stride says nothing
-    return t.data_ptr(), ld
+    ld, inner = t.stride()
+    if inner != 1 and shape[1] > 1:
+        raise N.PsError(N.PS_E_BAD_ARG, "%s: the columns of a row must be neighbours (stride %d)" % (name, inner))
+    return t.data_ptr(), ld if shape[0] > 1 else shape[1]      # (one row: its stride says nothing)
 
 
 def _f32(t, name, shape, like):
-    if tuple(t.shape) != shape or not t.is_contiguous() or t.device != like.device or str(t.dtype) != "torch.float32":
+    if tuple(t.shape) != shape or not t.is_contiguous() or t.get_device() != like.get_device() or str(t.dtype) != "torch.float32":
         raise N.PsError(N.PS_E_BAD_ARG, "%s: wanted a contiguous float32 tensor of shape %s on %s" % (name, shape, like.device))
     return t.data_ptr()
 
@@ -535,7 +534,7 @@ class _TowerLayer:
             if t is None:
                 raise N.PsError(N.PS_E_BAD_ARG, "activations are float32, bfloat16 or float16, not %s" % x.dtype)
             _TYPES[x.dtype] = t
-        if x.device.type != "cuda" or x.device.index != self.store.device:
+        if x.get_device() != self.store.device:
             raise N.PsError(N.PS_E_BAD_ARG, "x is on %s, the store on device %d" % (x.device, self.store.device))
         return t
 
