@@ -128,21 +128,24 @@ template <> struct Weights<float> {
 #define PS_WAIT_LOADS(n) PS_ORDERED(PS_WAIT_COUNTS(n))      // all but the last n loads have landed, too
 #define PS_BARRIER() PS_ORDERED(__builtin_amdgcn_s_barrier())
 
-// One BM x BN tile of the output per workgroup of 4 waves (2 x 2).  LDS rows are 128 bytes of the sum's axis (BK elements), 16-byte
+// One BM x BN tile of the output per workgroup of G groups of 4 waves (2 x 2 each).  LDS rows are 128 bytes of the sum's axis (BK elements), 16-byte
 // pieces exchanged by the row's low bits so that the fragment reads of 8 neighbouring rows touch all banks once.  The pieces of the
 // next AHEAD steps travel in registers while this step multiplies; two LDS buffers, one barrier a step (which waits for LDS alone, not for
 // the loads).
+// G > 1: the groups share the sum out -- for outputs of few tiles, whose chain of steps is what a call costs -- and add up through LDS, in
+// group order.
 // The product is formed transposed (weights as the first operand): a lane then holds 4 neighbouring columns of one row of y.
-template <typename T, int BM, int BN, int AHEAD>
-__global__ __launch_bounds__(256, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a, int tiles_n) {
+template <typename T, int BM, int BN, int AHEAD, int G>
+__global__ __launch_bounds__(256 * G, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a, int tiles_n) {
     typedef Mma<T> X;
     typedef typename X::frag frag;
     constexpr int CN = Chunk<T>::N, BK = X::BK, TILE = X::TILE, FM = BM / 2 / TILE, FN = BN / 2 / TILE, PA = BM * 8 / 256, PB = BN * 8 / 256;
-    __shared__ u32x4 sA[2][BM * 8], sB[2][BN * 8];
+    __shared__ u32x4 lds[G * 2 * (BM + BN) * 8];
     const int tile = xcd_tile(blockIdx.x, gridDim.x);
     const int64_t m0 = (int64_t)(tile / tiles_n) * BM;
     const int n0 = (tile % tiles_n) * BN;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+    const int tid = threadIdx.x & 255, grp = G > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+    u32x4(*sA)[BM * 8] = reinterpret_cast<u32x4(*)[BM * 8]>(lds + grp * 2 * (BM + BN) * 8), (*sB)[BN * 8] = reinterpret_cast<u32x4(*)[BN * 8]>(lds + grp * 2 * (BM + BN) * 8 + 2 * BM * 8);
     const T *pa[PA];
     const float *pb[PB];
     int dst_a[PA], dst_b[PB];
@@ -207,28 +210,52 @@ __global__ __launch_bounds__(256, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a, int
         }
     };
     // the step that K cuts off, if there is one, goes first: behind it no load hides behind a branch
-    const int full = a.K / BK, cut = a.K % BK ? 1 : 0, steps = full + cut;
-    if (cut) fetch_cut(full * BK); else fetch(0, 0);
+    const int full = a.K / BK, cut = a.K % BK ? 1 : 0, total = full + cut;
+    const int lo = total * grp / G, mine = total * (grp + 1) / G - lo, steps = (total + G - 1) / G;      // (with G > 1 every group has a step)
     if (!full) {                                 // nothing but the cut step
+        fetch_cut(0);
         put(0, 0);
         PS_WAIT_LDS(); PS_BARRIER();
         multiply(0);
     } else {
         // step s + p lies in buffer p and the next ones in registers or on their way.  The last steps ask again for what is there: the
         // loads are never behind a branch, so the waits know how many of them are younger than those they wait for.
-        auto ask = [&](int set, int step) { fetch(set, (step < steps ? step - cut : full - 1) * BK); };
+        auto ask = [&](int set, int s) { const int q = lo + (s < mine ? s : mine - 1); fetch(set, (q > cut ? q - cut : 0) * BK); };
         auto half = [&](int s, int p) {
             if (AHEAD > 1) ask(p, s + p + 2); else ask(0, s + p + 1);
-            multiply(p);
+            if (G == 1 || s + p < mine) multiply(p);
             put(AHEAD > 1 ? p ^ 1 : 0, p ^ 1);
             PS_WAIT_LDS(); PS_BARRIER();
         };
+        if (cut && grp == 0) fetch_cut(full * BK); else ask(0, 0);
         if (AHEAD > 1) ask(1, 1);
         put(0, 0);
         PS_WAIT_LDS(); PS_BARRIER();
         int s = 0;
         for (; s + 2 <= steps; s += 2) { half(s, 0); half(s, 1); }
         if (s < steps) half(s, 0);
+    }
+    if constexpr (G > 1) {
+        constexpr int AE = (int)(sizeof(acc[0][0]) / 4);
+        float *sums = reinterpret_cast<float *>(lds) + (wave * 64 + lane);
+        if (grp) {
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FM; ++j)
+#pragma unroll
+                    for (int e = 0; e < AE; ++e) sums[(((grp - 1) * FN + i) * FM + j) * AE * 256 + e * 256] = acc[i][j][e];
+        }
+        PS_WAIT_LDS(); PS_BARRIER();
+        if (grp) return;
+#pragma unroll
+        for (int g = 0; g < G - 1; ++g)
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FM; ++j)
+#pragma unroll
+                    for (int e = 0; e < AE; ++e) acc[i][j][e] += sums[((g * FN + i) * FM + j) * AE * 256 + e * 256];
     }
     // epilogue: groups of 4 neighbouring columns of one row
     constexpr int GR = (int)(sizeof(acc[0][0]) / 16);
@@ -955,11 +982,11 @@ int grid_ok(int64_t blocks) {
     return blocks * 256 < (1ll << 32) ? PS_OK : ps_set_err(PS_E_UNSUPPORTED, "the batch needs more workgroups than one launch has");
 }
 
-template <typename T, int BM, int BN, int AHEAD> int nt_go(const FcNtArgs &a, hipStream_t st) {
+template <typename T, int BM, int BN, int AHEAD, int G> int nt_go(const FcNtArgs &a, hipStream_t st) {
     const int tiles_n = cdiv(a.N, BN);
     const int64_t blocks = (int64_t)tiles_n * cdiv(a.M, BM);
     PSCHK(grid_ok(blocks));
-    hipLaunchKernelGGL((k_fc_nt<T, BM, BN, AHEAD>), dim3((unsigned)blocks), dim3(256), 0, st, a, tiles_n);
+    hipLaunchKernelGGL((k_fc_nt<T, BM, BN, AHEAD, G>), dim3((unsigned)blocks), dim3(256 * G), 0, st, a, tiles_n);
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
@@ -1008,18 +1035,19 @@ template <typename T, int FM> int few_go(const FcNtArgs &a, hipStream_t st) {
     HIPCHK(hipGetLastError());
     return PS_OK;
 }
-#ifndef A64
-#define A64 2
-#endif
-#ifndef A128
-#define A128 2
-#endif
+// Which kernel takes a product that k_fc_nt_big does not (us, few rows' kernel / 64 x 64 tiles).  Too few tiles for the chip leave the
+// tiles' chain of staged steps bare: bf16, 64 tiles, 128 x 2048 -> 2048: 11 / 18; 128 tiles, 1000 x 1000 -> 500: 12 / 10; f32, whose steps
+// are four times as long, 128 tiles, 2000 x 2000 -> 200: 35 / 42; 234 tiles, 2442 x 3688 -> 324: 116 / 76.
+// One tile a CU and a long sum, 16-bit: four groups of waves share it (1000 x 4096 -> 1024: 47 us by one group, 31 by four; with 512 tiles
+// 55 / 57; with a sum of 2048 21 / 20, of 1024 11 / 12; f32, bound by its matrix instructions, only loses: 26 / 34 for 4096 x 429 -> 512).
 template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
-    // below one 64 x 64 tile for each CU its chain of staged steps is what a call costs (bf16, 256 x 4096 -> 1024: 59 us, few rows' kernel 21;
-    // f32, 1000 x 275 -> 150: 13 / 6); at one a CU the tiles win (bf16, 1000 x 512 -> 1024: 11 / 16; 4096 x 429 -> 512: 15 / 60)
-    if (a.M <= 64 || (int64_t)cdiv(a.M, 64) * cdiv(a.N, 64) < 256) return a.M <= 16 ? few_go<T, 1>(a, st) : a.M <= 32 ? few_go<T, 2>(a, st) : few_go<T, 4>(a, st);
-    if ((int64_t)cdiv(a.M, 128) * cdiv(a.N, 128) >= 256) return nt_go<T, 128, 128, sizeof(T) == 4 ? A128 : 1>(a, st);
-    return nt_go<T, 64, 64, A64>(a, st);
+    const int64_t t128 = (int64_t)cdiv(a.M, 128) * cdiv(a.N, 128), t64 = (int64_t)cdiv(a.M, 64) * cdiv(a.N, 64);
+    if (a.M <= 64 || t64 < (sizeof(T) == 4 ? 200 : 100)) return a.M <= 16 ? few_go<T, 1>(a, st) : a.M <= 32 ? few_go<T, 2>(a, st) : few_go<T, 4>(a, st);
+    if (t128 >= 256) return nt_go<T, 128, 128, sizeof(T) == 4 ? 2 : 1, 1>(a, st);
+    if constexpr (sizeof(T) == 2) {
+        if (t64 <= 256 && a.K >= 2048) return nt_go<T, 64, 64, 2, 4>(a, st);
+    }
+    return nt_go<T, 64, 64, 2, 1>(a, st);
 }
 template <typename T, int BT> int tn_go(const FcTnArgs &a, hipStream_t st) {
     const int tiles_n = cdiv(a.N, BT), tiles = tiles_n * cdiv(a.K, BT);

@@ -254,7 +254,7 @@ def test_fc_res_forward_and_backward(pool, t, B, K, N_):
                                       (20000, 64, 1, R.SILU), (48, 4096, 1000, R.NONE), (1, 4096, 4096, R.SILU),
                                       (40000, 72, 200, R.GELU), (33000, 64, 256, R.RELU), (40000, 40, 296, R.NONE), (35003, 328, 77, R.SILU), (33100, 200, 128, R.GELU),
                                       (10950, 520, 776, R.GELU), (7301, 2056, 264, R.NONE), (4000, 1032, 2000, R.RELU),
-                                      (17000, 603, 517, R.GELU), (17001, 517, 603, R.NONE), (20001, 301, 333, R.SILU)])
+                                      (700, 2051, 700, R.SILU), (130, 4099, 640, R.GELU), (17000, 603, 517, R.GELU), (17001, 517, 603, R.NONE), (20001, 301, 333, R.SILU)])
 def test_fc_res_large(pool, t, B, K, N_, a):
     """sizes at which the split products, the large tiles and the few-row kernels run"""
     from ps_amd import native as N
