@@ -589,10 +589,12 @@ template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T 
 // of the sum inside a step is the same for both operands and otherwise free.  32-byte pieces are exchanged by a row key: the 8 rows
 // that 32 lanes of a transposing read touch lie in different banks.  The workgroups of the first row of tiles also multiply dz by a
 // fragment of ones: db, row K of the slab.
-// Two steps ahead in registers, as in k_fc_nt: the step that M cuts off goes first, columns behind K and N are read from the row's start
-// (their results go nowhere), and only a tile whose last 16-byte piece the width cuts off (CUT) loads element by element.
-template <typename T, int BT, bool CUT>
-__device__ __forceinline__ void fc_tn_tile(const FcTnArgs &a, int tiles_n, int split, int tile, u32x4 *lds) {
+// Two steps ahead in registers, as in k_fc_nt: the step that M cuts off goes first and is loaded element by element.  Columns behind K and
+// N are any values, their results go nowhere: whole pieces of them are read from the row's start, and a piece that the width cuts off
+// (edge) runs on into the next row -- so the step with the last row counts as cut off too.  NARROW: widths below a piece, whose pieces
+// could run past more than one row: every load element by element.
+template <typename T, int BT, bool NARROW>
+__device__ __forceinline__ void fc_tn_tile(const FcTnArgs &a, int tiles_n, int split, int tile, bool edge, u32x4 *lds) {
     typedef Mma<T> X;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int CN = Chunk<T>::N, ROWS = F32 ? 32 : 64, PER = BT / CN, P = ROWS * PER / 256, TILE = X::TILE, FK = BT / 2 / TILE, FN = BT / 2 / TILE;
@@ -602,7 +604,7 @@ __device__ __forceinline__ void fc_tn_tile(const FcTnArgs &a, int tiles_n, int s
     auto key = [](int row) { return F32 ? 0 : BT == 128 ? row & 7 : (row >> 1) & 3; };
     // this part's rows: whole steps, dealt evenly
     const int64_t all = ((int64_t)a.M + ROWS - 1) / ROWS, s_lo = all * split / a.nsplit, s_hi = all * (split + 1) / a.nsplit;
-    const int cut = s_hi * ROWS > a.M ? 1 : 0, steps = (int)(s_hi - s_lo), full = steps - cut;
+    const int cut = s_hi * ROWS > a.M || (edge && s_hi == all) ? 1 : 0, steps = (int)(s_hi - s_lo), full = steps - cut;
     Chunk<T> rx[2][P], rd[2][P];
     int dst[P], cx[P], cd[P];
 #pragma unroll
@@ -610,14 +612,14 @@ __device__ __forceinline__ void fc_tn_tile(const FcTnArgs &a, int tiles_n, int s
         const int q = tid + i * 256, row = q / PER, c = q % PER;
         dst[i] = row * PER + (c ^ (key(row) << 1));
         cx[i] = k0 + c * CN; cd[i] = n0 + c * CN;
-        if (!CUT) { cx[i] = cx[i] < a.K ? cx[i] : 0; cd[i] = cd[i] < a.N ? cd[i] : 0; }
+        if (!NARROW) { cx[i] = cx[i] < a.K ? cx[i] : 0; cd[i] = cd[i] < a.N ? cd[i] : 0; }
     }
     auto fetch = [&](int set, int64_t step) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int64_t m = (s_lo + step) * ROWS + (tid + i * 256) / PER;
             const T *px = (const T *)a.X + m * a.ldx, *pd = (const T *)a.D + m * a.ldd;
-            if constexpr (CUT) { rx[set][i].load(px, cx[i], a.K); rd[set][i].load(pd, cd[i], a.N); }
+            if constexpr (NARROW) { rx[set][i].load(px, cx[i], a.K); rd[set][i].load(pd, cd[i], a.N); }
             else {
                 rx[set][i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(px + cx[i]);
                 rd[set][i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(pd + cd[i]);
@@ -745,9 +747,9 @@ __global__ __launch_bounds__(256, BT == 64 ? 3 : 2) void k_fc_tn(FcTnArgs a, int
     constexpr int CN = Chunk<T>::N;
     __shared__ u32x4 lds[4 * (sizeof(T) == 4 ? 32 : 64) * BT / CN];
     const int id = xcd_tile(blockIdx.x, gridDim.x), split = id / tiles, tile = id % tiles;
-    const bool cut = (a.K % CN && (tile / tiles_n + 1) * BT > a.K) || (a.N % CN && (tile % tiles_n + 1) * BT > a.N);
-    if (cut) fc_tn_tile<T, BT, true>(a, tiles_n, split, tile, lds);
-    else fc_tn_tile<T, BT, false>(a, tiles_n, split, tile, lds);
+    const bool edge = (a.K % CN && (tile / tiles_n + 1) * BT > a.K) || (a.N % CN && (tile % tiles_n + 1) * BT > a.N);
+    if (a.K < CN || a.N < CN) fc_tn_tile<T, BT, true>(a, tiles_n, split, tile, edge, lds);
+    else fc_tn_tile<T, BT, false>(a, tiles_n, split, tile, edge, lds);
 }
 
 // The transposing LDS read.  As a function of a restrict pointer: the compiler then knows what it reads, and does not wait for every load
@@ -1000,15 +1002,16 @@ int ag_t(int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void
 }
 // Whether and how a product takes k_fc_nt_big.  Its loads want 16-byte pieces and its offsets 31 bits; rows that start elsewhere are
 // copied first, which a product of 256 columns or more pays for (bf16, 20000 x 1001 -> 1001 relu: 118 us without, 79 with).
-// 128 columns cost 0.6 of 256 (measured on full chips), so they win where they halve the rounds of the 256 CUs; below half a round the
-// small tiles win.
+// 128 columns cost 0.6 of 256 (measured on full chips), so they win where they halve the rounds of the 256 CUs; below half a round of
+// 128 columns the small tiles win (4096 x 1024 -> 512, 64 tiles: 20 us by 256 x 128, 14 by 64 x 64), below a quarter for long sums
+// (500 x 4096 -> 4096, 64 tiles: 64 / 132; 1000 x 4096 -> 1024, 32 tiles: 53 / 31).
 struct NtPlan { int bn = 0; bool pack = false; };
 NtPlan nt_plan(int type, const FcNtArgs &a) {
     NtPlan p;
     if (type == PS_T_F32 || a.K > (1 << 21)) return p;
     p.pack = (uintptr_t)a.A % 16 || a.lda % 8 || a.lda > (1 << 21);
     const int64_t tm = cdiv(a.M, BIG_M), t2 = tm * cdiv(a.N, 256), t1 = tm * cdiv(a.N, 128);
-    if (t1 < 128 || t1 >= (1 << 30) || (p.pack && a.N < 256)) return p;
+    if (t1 < (a.K >= 4096 ? 64 : 128) || t1 >= (1 << 30) || (p.pack && a.N < 256)) return p;
     p.bn = 10 * cdiv(t2, 256) <= 6 * cdiv(t1, 256) ? 256 : 128;
     return p;
 }
@@ -1038,12 +1041,14 @@ template <typename T, int FM> int few_go(const FcNtArgs &a, hipStream_t st) {
 // Which kernel takes a product that k_fc_nt_big does not (us, few rows' kernel / 64 x 64 tiles).  Too few tiles for the chip leave the
 // tiles' chain of staged steps bare: bf16, 64 tiles, 128 x 2048 -> 2048: 11 / 18; 128 tiles, 1000 x 1000 -> 500: 12 / 10; f32, whose steps
 // are four times as long, 128 tiles, 2000 x 2000 -> 200: 35 / 42; 234 tiles, 2442 x 3688 -> 324: 116 / 76.
+// 128 x 128 tiles only where they fill the two a CU twice (f32: 8192 x 2048 -> 2048 592 by 64, 533 by 128; 20000 x 300 -> 300 46 / 53;
+// 2442 x 324 -> 3688 78 / 92).
 // One tile a CU and a long sum, 16-bit: four groups of waves share it (1000 x 4096 -> 1024: 47 us by one group, 31 by four; with 512 tiles
 // 55 / 57; with a sum of 2048 21 / 20, of 1024 11 / 12; f32, bound by its matrix instructions, only loses: 26 / 34 for 4096 x 429 -> 512).
 template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
     const int64_t t128 = (int64_t)cdiv(a.M, 128) * cdiv(a.N, 128), t64 = (int64_t)cdiv(a.M, 64) * cdiv(a.N, 64);
     if (a.M <= 64 || t64 < (sizeof(T) == 4 ? 200 : 100)) return a.M <= 16 ? few_go<T, 1>(a, st) : a.M <= 32 ? few_go<T, 2>(a, st) : few_go<T, 4>(a, st);
-    if (t128 >= 256) return nt_go<T, 128, 128, sizeof(T) == 4 ? 2 : 1, 1>(a, st);
+    if (t128 >= 1024) return nt_go<T, 128, 128, sizeof(T) == 4 ? 2 : 1, 1>(a, st);
     if constexpr (sizeof(T) == 2) {
         if (t64 <= 256 && a.K >= 2048) return nt_go<T, 64, 64, 2, 4>(a, st);
     }
@@ -1107,7 +1112,7 @@ void fc_tn_plan(int type, FcTnArgs &a) {
     a.nbias = 1;
     for (a.tile = 128;; a.tile = 64) {
         const int64_t tiles = (int64_t)cdiv(a.N, a.tile) * cdiv(a.K, a.tile);
-        int64_t s = (512 + tiles - 1) / tiles;
+        int64_t s = 512 / tiles;                 // (rounded down: one workgroup too many is a round too many)
         if (s > st / 4) s = st / 4;
         a.nsplit = (int)(s < 1 ? 1 : s);
         if (a.tile == 64 || st >= 8 * a.nsplit) return;
