@@ -340,7 +340,8 @@ int ps_dense_update(ps_store_t *s, int layer);
  * except a call that has to enlarge the store's workspace.
  * HIP graphs: a call may be recorded (on a capturing stream adopted with
  * ps_store_set_stream) once the same shapes have run eagerly -- the workspace
- * does not grow while recording, PS_E_STATE -- and with grad_dev given: the
+ * does not grow while recording, PS_E_STATE, nor may a fused training step still
+ * be waiting to be joined (ps_store_sync first) -- and with grad_dev given: the
  * pending gradient's count lives on the host, so a call that would add to it is
  * refused while recording, PS_E_UNSUPPORTED.  The workspace is the store's: replays
  * of its graphs are calls on the store, one at a time like all of them. */

@@ -8,7 +8,8 @@ public final class NativeKVStore implements AutoCloseable {
     static { System.loadLibrary("ps_amd_jni"); }       // ps_jni.cpp, linked against libps_amd.so
 
     // constants of include/ps_native.h
-    public static final int ACT_NONE = 0, ACT_RELU = 1, ACT_SIGMOID = 2;
+    public static final int ACT_NONE = 0, ACT_RELU = 1, ACT_SIGMOID = 2, ACT_GELU = 3, ACT_SILU = 4;
+    public static final int T_F32 = 0, T_BF16 = 1, T_F16 = 2;
     public static final int GRAD_COMPAT = 0, GRAD_INTENDED = 1;
     public static final int SUM_AUTO = 0, SUM_SEQUENTIAL = 1, SUM_CHUNKED = 2;
     public static final int ROUTE_ID_MOD = 0, ROUTE_JAVA_STRING = 1;
@@ -66,6 +67,16 @@ public final class NativeKVStore implements AutoCloseable {
     /** FcLayer.forward / backward (layer/FcLayer.java:74-110); backward leaves dW, db in the store's pending sums */
     public native void fcForward(int layer, int act, long xDev, int ldx, int B, long yDev, int ldy);
     public native void fcBackward(int layer, int act, long xDev, int ldx, long yDev, int ldy, long deltaDev, int ldd, int B, long dxDev, int lddx);
+    /** the residual tower: layer normalisation and FC with bias, activation and residual; type T_*, leading dimensions in elements of it, 0 for
+     *  an operand that is not given; gradDev 0: into the store's pending sums (lnUpdate / denseUpdate apply them) */
+    public native void createLn(int layer, int dims);
+    public native void lnForward(int layer, int type, long xDev, long ldx, int B, float eps, long yDev, long ldy, long statsDev);
+    public native void lnBackward(int layer, int type, long xDev, long ldx, long statsDev, long dyDev, long lddy, int B, long skipDev, long ldskip,
+                                  long dxDev, long lddx, long gradDev);
+    public native void lnUpdate(int layer);
+    public native void fcResForward(int layer, int type, int act, long xDev, long ldx, int B, long rDev, long ldr, long zDev, long ldz, long yDev, long ldy);
+    public native void fcResBackward(int layer, int type, int act, long xDev, long ldx, long zDev, long ldz, long dyDev, long lddy, int B,
+                                     long skipDev, long ldskip, long dxDev, long lddx, long gradDev);
     /** KVStore.update(Map) + clear for the dense tensors; layer < 0: all (store/KVStore.java:240-277) */
     public native void denseUpdate(int layer);
     public native void sync();

@@ -230,6 +230,37 @@ JNIEXPORT void JNICALL Java_store_NativeKVStore_fcBackward(JNIEnv *env, jobject 
     fail(env, ps_fc_backward(S(env, self), layer, act, reinterpret_cast<const float *>(xDev), ldx, reinterpret_cast<const float *>(yDev), ldy,
                              reinterpret_cast<float *>(deltaDev), ldd, B, reinterpret_cast<float *>(dxDev), lddx));
 }
+JNIEXPORT void JNICALL Java_store_NativeKVStore_createLn(JNIEnv *env, jobject self, jint layer, jint dims) {
+    fail(env, ps_store_create_ln(S(env, self), layer, dims));
+}
+JNIEXPORT void JNICALL Java_store_NativeKVStore_lnForward(JNIEnv *env, jobject self, jint layer, jint type, jlong xDev, jlong ldx, jint B, jfloat eps,
+                                                          jlong yDev, jlong ldy, jlong statsDev) {
+    fail(env, ps_ln_forward(S(env, self), layer, type, reinterpret_cast<const void *>(xDev), ldx, B, eps, reinterpret_cast<void *>(yDev), ldy,
+                            reinterpret_cast<float *>(statsDev)));
+}
+JNIEXPORT void JNICALL Java_store_NativeKVStore_lnBackward(JNIEnv *env, jobject self, jint layer, jint type, jlong xDev, jlong ldx, jlong statsDev,
+                                                           jlong dyDev, jlong lddy, jint B, jlong skipDev, jlong ldskip, jlong dxDev, jlong lddx,
+                                                           jlong gradDev) {
+    fail(env, ps_ln_backward(S(env, self), layer, type, reinterpret_cast<const void *>(xDev), ldx, reinterpret_cast<const float *>(statsDev),
+                             reinterpret_cast<const void *>(dyDev), lddy, B, reinterpret_cast<const void *>(skipDev), ldskip,
+                             reinterpret_cast<void *>(dxDev), lddx, reinterpret_cast<float *>(gradDev)));
+}
+JNIEXPORT void JNICALL Java_store_NativeKVStore_lnUpdate(JNIEnv *env, jobject self, jint layer) {
+    const int rc = ps_ln_update(S(env, self), layer);
+    if (rc != PS_MISSING) fail(env, rc);                  // nothing pending: as denseUpdate
+}
+JNIEXPORT void JNICALL Java_store_NativeKVStore_fcResForward(JNIEnv *env, jobject self, jint layer, jint type, jint act, jlong xDev, jlong ldx, jint B,
+                                                             jlong rDev, jlong ldr, jlong zDev, jlong ldz, jlong yDev, jlong ldy) {
+    fail(env, ps_fc_res_forward(S(env, self), layer, type, act, reinterpret_cast<const void *>(xDev), ldx, B, reinterpret_cast<const void *>(rDev), ldr,
+                                reinterpret_cast<void *>(zDev), ldz, reinterpret_cast<void *>(yDev), ldy));
+}
+JNIEXPORT void JNICALL Java_store_NativeKVStore_fcResBackward(JNIEnv *env, jobject self, jint layer, jint type, jint act, jlong xDev, jlong ldx,
+                                                              jlong zDev, jlong ldz, jlong dyDev, jlong lddy, jint B, jlong skipDev, jlong ldskip,
+                                                              jlong dxDev, jlong lddx, jlong gradDev) {
+    fail(env, ps_fc_res_backward(S(env, self), layer, type, act, reinterpret_cast<const void *>(xDev), ldx, reinterpret_cast<const void *>(zDev), ldz,
+                                 reinterpret_cast<const void *>(dyDev), lddy, B, reinterpret_cast<const void *>(skipDev), ldskip,
+                                 reinterpret_cast<void *>(dxDev), lddx, reinterpret_cast<float *>(gradDev)));
+}
 JNIEXPORT void JNICALL Java_store_NativeKVStore_denseUpdate(JNIEnv *env, jobject self, jint layer) {
     const int rc = ps_dense_update(S(env, self), layer);
     if (rc != PS_MISSING) fail(env, rc);                  // nothing pending: KVStore.update over an empty sum map is a no-op

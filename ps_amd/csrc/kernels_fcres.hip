@@ -35,8 +35,7 @@ template <> struct Mma<float> {        // a fragment holds 4 steps of 2: the lan
 // rounding of 1 + erf in f32), whose e^(-z^2 / 2) the slope needs anyway.  About 20 instruction slots with one reciprocal and one
 // exponential, a third of the library's erff -- in the epilogue of a product nothing hides them.
 __device__ __forceinline__ float normal_tail(float z, float &e) {
-    const float x = fabsf(z);
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, x, 1.f));
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
     e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);                       // e^(-z^2 / 2)
     float p = fmaf(1.061405429f, t, -1.453152027f);
     p = fmaf(p, t, 1.421413741f);
@@ -52,20 +51,22 @@ template <int NV> __device__ __forceinline__ void act_apply(float (&v)[NV], int 
         for (int j = 0; j < NV; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];        // (a NaN stays one)
     } else if (act == PS_ACT_GELU) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = fmaf(-fabsf(v[j]), normal_tail(v[j], e), fmaxf(v[j], 0.f));      // z Phi(z) = max(z, 0) - |z| Q(|z|)
+        for (int j = 0; j < NV; ++j)             // z Phi(z) = max(z, 0) - |z| Q(|z|), and Q(64) is 0 (so is Q(infinity) times it)
+            v[j] = fmaf(-fminf(fabsf(v[j]), 64.f), normal_tail(v[j], e), fmaxf(v[j], 0.f));
     } else if (act == PS_ACT_SILU) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) v[j] *= logistic(v[j]);
     }
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
+    const float x = fminf(fmaxf(z, -128.f), 128.f);      // (beyond, both slopes are 0 and 1 to the last bit, and infinity times 0 is not)
     if (act == PS_ACT_GELU) {
         float e;
         const float q = normal_tail(z, e);
-        return fmaf(z * 0.39894228f, e, z < 0.f ? q : 1.f - q);
+        return fmaf(x * 0.39894228f, e, z < 0.f ? q : 1.f - q);
     }
     const float p = logistic(z);
-    return p * fmaf(z, 1.f - p, 1.f);
+    return p * fmaf(x, 1.f - p, 1.f);
 }
 
 // workgroup -> tile so that an XCD (workgroup id mod 8) owns a contiguous range of tiles: its L2 then serves the tiles' shared rows

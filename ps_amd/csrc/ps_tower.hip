@@ -70,6 +70,13 @@ int check_act(int act) {
     return PS_OK;
 }
 
+// store_enter; a fused step's last join cannot be recorded (its event lies outside the graph) and must not be lost either
+int tower_enter(ps_store *s) {
+    if (s->pending_ev && stream_is_capturing(s->stream))
+        return ps_set_err(PS_E_STATE, "a training step is still to be joined: call ps_store_sync before a graph is recorded");
+    return store_enter(s);
+}
+
 // `need` bytes of workspace for one call; its contents are dead when the call's launches are done
 int workspace(ps_store *s, size_t need, char **out) {
     ps_store::TowerWs &w = s->tower;
@@ -121,7 +128,7 @@ extern "C" int ps_ln_forward(ps_store_t *s, int layer, int type, const void *x_d
     PSCHK(check_mat(y, B, es));
     PSCHK(check_out(y, x, B, es, true));
     PSCHK(check_f32("stats_dev", stats_dev, 2ll * B, {x, y}, B, es));
-    PSCHK(store_enter(s));
+    PSCHK(tower_enter(s));
     LnFwdArgs a;
     a.x = x_dev; a.ldx = ldx; a.y = y_dev; a.ldy = ldy; a.gamma = p->W; a.beta = p->W + p->ldw; a.stats = stats_dev;
     a.B = B; a.D = p->N; a.eps = eps;
@@ -144,7 +151,7 @@ extern "C" int ps_ln_backward(ps_store_t *s, int layer, int type, const void *x_
     PSCHK(check_out(dx, sk, B, es, true));
     PSCHK(check_f32("grad_dev", grad_dev, 2ll * D, {x, dy, sk, dx}, B, es));
     PSCHK(check_f32("stats_dev", stats_dev, 2ll * B, {dx}, B, es));
-    PSCHK(store_enter(s));
+    PSCHK(tower_enter(s));
     float *dst;
     int accum;
     PSCHK(grad_target(s, *p, grad_dev, &dst, &accum));
@@ -202,7 +209,7 @@ extern "C" int ps_fc_res_forward(ps_store_t *s, int layer, int type, int act, co
     PSCHK(check_out(y, z, B, es));
     PSCHK(check_out(z, x, B, es));
     PSCHK(check_out(z, r, B, es));
-    PSCHK(store_enter(s));
+    PSCHK(tower_enter(s));
     FcNtArgs a;
     a.A = x_dev; a.lda = ldx; a.W = p->Wt; a.ldw = p->Kpad; a.bias = p->W + (size_t)p->K * p->ldw; a.R = r_dev; a.ldr = r_dev ? ldr : 0;
     a.Z = z_dev; a.ldz = z_dev ? ldz : 0; a.Y = y_dev; a.ldy = ldy; a.M = B; a.N = p->N; a.K = p->K; a.act = act;
@@ -231,7 +238,7 @@ extern "C" int ps_fc_res_backward(ps_store_t *s, int layer, int type, int act, c
     for (const Mat *m : {&x, &z, &dy}) PSCHK(check_out(dx, *m, B, es));
     PSCHK(check_out(dx, sk, B, es, true));
     PSCHK(check_f32("grad_dev", grad_dev, (int64_t)(K + 1) * N, {x, z, dy, sk, dx}, B, es));
-    PSCHK(store_enter(s));
+    PSCHK(tower_enter(s));
     hipStream_t st = s->stream;
     float *dst;
     int accum;

@@ -308,6 +308,36 @@ def test_fc_bad_values_stay_in_their_row(pool, t, B):
     within(gr.get(), grad, tg, "gradient")
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_activations_at_their_ends(pool, t):
+    """z from far below to far above, the borders, infinities and a NaN, through a product by one: values and slopes"""
+    from ps_amd import native as N
+    L, kv = N.lib(), pool.kv
+    kv.create_fc(0, 1, 1)
+    kv.put("fc0.weights", [1.0]); kv.put("fc0.bias", [0.0])
+    z = np.array([-np.inf, -1e4, -200, -100, -64, -30, -13, -6, -4, -3, -1, -1e-3, -1e-7, 0, 1e-7, 1e-3, 0.5, 1, 3, 4, 6, 13, 30, 64, 100, 200, 1e4, np.inf, np.nan])
+    B = z.size
+    zr, y, dy = pool.rows(t, B, 1, values=z[:, None]), pool.rows(t, B, 1), pool.rows(t, B, 1, values=np.ones((B, 1)))
+    dx, g = pool.rows(t, B, 1), pool.rows(R.F32, 2, 1)
+    zv = R.rounded(z, t)
+    fin = np.isfinite(zv)
+    for a in (R.RELU, R.GELU, R.SILU):
+        N.check(L.ps_fc_res_forward(kv.h, 0, t, a, zr.p, 1, B, None, 0, None, 0, y.p, 1))
+        N.check(L.ps_fc_res_backward(kv.h, 0, t, a, zr.p, 1, zr.p, 1, dy.p, 1, B, None, 0, dx.p, 1, g.p))
+        got, slope = y.get()[:, 0], dx.get()[:, 0]
+        with np.errstate(all="ignore"):
+            want, dwant = R.act(zv, a), R.act_grad(zv, a)
+        tol = (0 if a == R.RELU else 8 * R.U) * np.abs(zv[fin]) + R.store_tol(np.abs(want[fin]) * 1.001, t) + 1e-37
+        within(got[fin], want[fin], tol, "act %d" % a)
+        tol = (0 if a == R.RELU else 14 * R.U) * (1 + np.minimum(np.abs(zv[fin]), 8)) + R.store_tol(np.abs(dwant[fin]) * 1.001, t)
+        within(slope[fin], dwant[fin], tol, "slope %d" % a)
+        up = zv == np.inf
+        assert (got[up] == np.inf).all() and (slope[up] == 1).all() and np.isnan(got[-1])
+        if a != R.SILU:
+            assert (got[zv == -np.inf] == 0).all()
+        assert (slope[zv == -np.inf] == 0).all()
+
+
 def test_pending_gradients_updaters_and_keys(pool, orc):
     """two backward calls add up in the store's pending gradients (KVStore.sum), dense_update divides by their number and runs every
     tensor's own updater; the keys are read, written, pushed and sized like the FC layers'"""
@@ -514,6 +544,42 @@ def test_recorded_and_replayed(pool, t):
                 np.testing.assert_array_equal(s[k].raw().view(np.uint8), replay[k].view(np.uint8), err_msg=k)
     for e in execs:
         hip("hipGraphExecDestroy", e)
+    for r in pool.all:
+        r.free()
+    pool.all = []
+    kv.close()
+    hip("hipStreamDestroy", stream)
+
+
+def test_recording_behind_a_training_step(pool):
+    """a fused step's last join lies outside a graph: the call is refused while recording, the join is not lost, and what follows is whole"""
+    import ps_amd
+    from ps_amd import native as N
+    L, kv, hip = N.lib(), pool.kv, Hip()
+    F, D, X, V, B = 4, 8, 5, 50, 512
+    rng = np.random.default_rng(3)
+    kv.create_embedding([V] * F, D)
+    m = ps_amd.DNN.buildModel(F, D, X, [32, 16, 1], store=kv, max_batch=B)
+    kv.create_ln(0, 32)
+    x, y = pool.rows(R.F32, B, 32, values=rng.standard_normal((B, 32))), pool.rows(R.F32, B, 32)
+    stream = C.c_void_p()
+    hip("hipStreamCreateWithFlags", C.byref(stream), 1)
+    kv.set_stream(stream)
+    b = ps_amd.DeviceBatch(kv, rng.integers(0, V, (B, F)), rng.standard_normal((B, X)), (rng.random(B) < 0.3).astype(f32))
+    for _ in range(3):
+        m.train_async(b)
+    hip("hipStreamBeginCapture", stream, 2)
+    rc = L.ps_ln_forward(kv.h, 0, R.F32, x.p, 32, B, EPS, y.p, 32, None)
+    g = C.c_void_p()
+    hip("hipStreamEndCapture", stream, C.byref(g))
+    assert rc in (N.PS_OK, N.PS_E_STATE)                          # (a store that joins by events has nothing left to join)
+    kv.sync()
+    N.check(L.ps_ln_forward(kv.h, 0, R.F32, x.p, 32, B, EPS, y.p, 32, None))
+    xv = x.get()
+    within(y.get(), R.ln_forward(xv, 1.0, 0.0, f32(EPS))[0], R.ln_forward_tol(xv, np.ones(32), np.zeros(32), f32(EPS), R.F32)[0], "y")
+    assert np.isfinite(m.train(b))
+    b.close()
+    m.close()
     for r in pool.all:
         r.free()
     pool.all = []
