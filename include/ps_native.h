@@ -333,7 +333,7 @@ int ps_dense_update(ps_store_t *s, int layer);
  * is rounded once.
  * x_dev etc. are [B][width] with a row stride ld >= width in ELEMENTS of the type,
  * any stride and any alignment of the element's own size (16-byte aligned rows
- * are fastest); nothing behind a row's width is read or written.  No ones column.
+ * are fastest); what lies behind a row's width has no effect and is not written.  No ones column.
  * Activations: PS_ACT_NONE, RELU, GELU, SILU (SIGMOID is the head's: PS_E_UNSUPPORTED).
  * Outputs may not overlap inputs, except where a call says so: PS_E_BAD_ARG.
  * Everything is enqueued on the store's stream; nothing waits for the device

@@ -137,12 +137,10 @@ template <> struct Weights<float> {
 // group order.
 // The product is formed transposed (weights as the first operand): a lane then holds 4 neighbouring columns of one row of y.
 template <typename T, int BM, int BN, int AHEAD, int G>
-__global__ __launch_bounds__(256 * G, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a, int tiles_n) {
+__device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int tile, u32x4 *lds) {
     typedef Mma<T> X;
     typedef typename X::frag frag;
     constexpr int CN = Chunk<T>::N, BK = X::BK, TILE = X::TILE, FM = BM / 2 / TILE, FN = BN / 2 / TILE, PA = BM * 8 / 256, PB = BN * 8 / 256;
-    __shared__ u32x4 lds[G * 2 * (BM + BN) * 8];
-    const int tile = xcd_tile(blockIdx.x, gridDim.x);
     const int64_t m0 = (int64_t)(tile / tiles_n) * BM;
     const int n0 = (tile % tiles_n) * BN;
     const int tid = threadIdx.x & 255, grp = G > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
@@ -292,6 +290,11 @@ __global__ __launch_bounds__(256 * G, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a,
                 o.store(y, n, a.N);
             }
     }
+}
+template <typename T, int BM, int BN, int AHEAD, int G>
+__global__ __launch_bounds__(256 * G, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a, int tiles_n) {
+    __shared__ u32x4 lds[G * 2 * (BM + BN) * 8];
+    fc_nt_tile<T, BM, BN, AHEAD, G>(a, tiles_n, xcd_tile(blockIdx.x, gridDim.x), lds);
 }
 
 // Few rows (or few tiles): one workgroup of 16 waves per 16 columns and 16 FM rows.  The waves share out the sum in steps and take their
@@ -743,14 +746,28 @@ __device__ __forceinline__ void fc_tn_tile(const FcTnArgs &a, int tiles_n, int s
         if (do_bias && lg == 0) leave((size_t)a.K * a.N + n, accb[j][0]);
     }
 }
-template <typename T, int BT>
-__global__ __launch_bounds__(256, BT == 64 ? 3 : 2) void k_fc_tn(FcTnArgs a, int tiles_n, int tiles) {
+template <typename T, int BT> constexpr int kTnLds = 4 * (sizeof(T) == 4 ? 32 : 64) * BT / Chunk<T>::N;
+template <typename T, int BT> __device__ __forceinline__ void fc_tn_part(const FcTnArgs &a, int tiles_n, int tiles, int id, u32x4 *lds) {
     constexpr int CN = Chunk<T>::N;
-    __shared__ u32x4 lds[4 * (sizeof(T) == 4 ? 32 : 64) * BT / CN];
-    const int id = xcd_tile(blockIdx.x, gridDim.x), split = id / tiles, tile = id % tiles;
+    const int split = id / tiles, tile = id % tiles;
     const bool edge = (a.K % CN && (tile / tiles_n + 1) * BT > a.K) || (a.N % CN && (tile % tiles_n + 1) * BT > a.N);
     if (a.K < CN || a.N < CN) fc_tn_tile<T, BT, true>(a, tiles_n, split, tile, edge, lds);
     else fc_tn_tile<T, BT, false>(a, tiles_n, split, tile, edge, lds);
+}
+template <typename T, int BT>
+__global__ __launch_bounds__(256, BT == 64 ? 3 : 2) void k_fc_tn(FcTnArgs a, int tiles_n, int tiles) {
+    __shared__ u32x4 lds[kTnLds<T, BT>];
+    fc_tn_part<T, BT>(a, tiles_n, tiles, xcd_tile(blockIdx.x, gridDim.x), lds);
+}
+// dW's tiles and, behind them, dx's, in one launch: where neither fills the chip they run side by side, and there is one start and one end
+// less (two launches / one: bf16, 4096 x 512 -> 256 with relu 24.7 / 21.5 us, 4096 x 429 -> 512 with GELU 30.2 / 25.4; f32 40.8 / 35.4 and
+// 57.2 / 52.0; where the chip is full no difference: f32, 16384 x 429 -> 512 169.7 / 168.2, bf16, 100000 x 64 -> 64 38.2 / 38.5).
+template <typename T>
+__global__ __launch_bounds__(256, 3) void k_fc_both(FcTnArgs t, int t_tiles_n, int t_tiles, int t_blocks, FcNtArgs a, int tiles_n) {
+    __shared__ u32x4 lds[kTnLds<T, 64> > 2 * 128 * 8 ? kTnLds<T, 64> : 2 * 128 * 8];
+    const int id = blockIdx.x;
+    if (id < t_blocks) fc_tn_part<T, 64>(t, t_tiles_n, t_tiles, xcd_tile(id, t_blocks), lds);
+    else fc_nt_tile<T, 64, 64, 2, 1>(a, tiles_n, xcd_tile(id - t_blocks, gridDim.x - t_blocks), lds);
 }
 
 // The transposing LDS read.  As a function of a restrict pointer: the compiler then knows what it reads, and does not wait for every load
@@ -1046,12 +1063,19 @@ template <typename T, int FM> int few_go(const FcNtArgs &a, hipStream_t st) {
 // 2442 x 324 -> 3688 78 / 92).
 // One tile a CU and a long sum, 16-bit: four groups of waves share it (1000 x 4096 -> 1024: 47 us by one group, 31 by four; with 512 tiles
 // 55 / 57; with a sum of 2048 21 / 20, of 1024 11 / 12; f32, bound by its matrix instructions, only loses: 26 / 34 for 4096 x 429 -> 512).
-template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
+enum NtKind { NT_FEW, NT_128, NT_64_SPLIT, NT_64 };
+template <typename T> NtKind nt_kind(const FcNtArgs &a) {
     const int64_t t128 = (int64_t)cdiv(a.M, 128) * cdiv(a.N, 128), t64 = (int64_t)cdiv(a.M, 64) * cdiv(a.N, 64);
-    if (a.M <= 64 || t64 < (sizeof(T) == 4 ? 200 : 100)) return a.M <= 16 ? few_go<T, 1>(a, st) : a.M <= 32 ? few_go<T, 2>(a, st) : few_go<T, 4>(a, st);
-    if (t128 >= 1024) return nt_go<T, 128, 128, sizeof(T) == 4 ? 2 : 1, 1>(a, st);
+    if (a.M <= 64 || t64 < (sizeof(T) == 4 ? 200 : 100)) return NT_FEW;
+    if (t128 >= 1024) return NT_128;
+    return sizeof(T) == 2 && t64 <= 256 && a.K >= 2048 ? NT_64_SPLIT : NT_64;
+}
+template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
+    const NtKind k = nt_kind<T>(a);
+    if (k == NT_FEW) return a.M <= 16 ? few_go<T, 1>(a, st) : a.M <= 32 ? few_go<T, 2>(a, st) : few_go<T, 4>(a, st);
+    if (k == NT_128) return nt_go<T, 128, 128, sizeof(T) == 4 ? 2 : 1, 1>(a, st);
     if constexpr (sizeof(T) == 2) {
-        if (t64 <= 256 && a.K >= 2048) return nt_go<T, 64, 64, 2, 4>(a, st);
+        if (k == NT_64_SPLIT) return nt_go<T, 64, 64, 2, 4>(a, st);
     }
     return nt_go<T, 64, 64, 2, 1>(a, st);
 }
@@ -1119,9 +1143,8 @@ void fc_tn_plan(int type, FcTnArgs &a) {
         if (a.tile == 64 || st >= 8 * a.nsplit) return;
     }
 }
-int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st) {
-    if (a.tile == 256) PSCHK(type == PS_T_BF16 ? tn_big<__bf16>(a, st) : tn_big<_Float16>(a, st));
-    else PSCHK(type == PS_T_F32 ? tn_t<float>(a, st) : type == PS_T_BF16 ? tn_t<__bf16>(a, st) : tn_t<_Float16>(a, st));
+namespace {
+int tn_reduce(const FcTnArgs &a, hipStream_t st) {
     if (a.nsplit * a.nbias == 1) return PS_OK;               // (the kernel has left the result itself)
     const int64_t n = (int64_t)a.K * a.N;
     const int db = cdiv(a.N, 64);
@@ -1136,4 +1159,26 @@ int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st) {
     }
     HIPCHK(hipGetLastError());
     return PS_OK;
+}
+template <typename T> int both_go(const FcNtArgs &a, const FcTnArgs &t, hipStream_t st) {
+    const int tn = cdiv(t.N, 64), tt = tn * cdiv(t.K, 64), tiles_n = cdiv(a.N, 64);
+    const int64_t tb = (int64_t)tt * t.nsplit, blocks = tb + (int64_t)tiles_n * cdiv(a.M, 64);
+    PSCHK(grid_ok(blocks));
+    hipLaunchKernelGGL((k_fc_both<T>), dim3((unsigned)blocks), dim3(256), 0, st, t, tn, tt, (int)tb, a, tiles_n);
+    HIPCHK(hipGetLastError());
+    return PS_OK;
+}
+}  // namespace
+
+int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st) {
+    if (a.tile == 256) PSCHK(type == PS_T_BF16 ? tn_big<__bf16>(a, st) : tn_big<_Float16>(a, st));
+    else PSCHK(type == PS_T_F32 ? tn_t<float>(a, st) : type == PS_T_BF16 ? tn_t<__bf16>(a, st) : tn_t<_Float16>(a, st));
+    return tn_reduce(a, st);
+}
+bool fc_both_ok(int type, const FcNtArgs &a, const FcTnArgs &t) {
+    return t.tile == 64 && !nt_plan(type, a).bn && (type == PS_T_F32 ? nt_kind<float>(a) : nt_kind<__bf16>(a)) == NT_64;
+}
+int launch_fc_both(int type, const FcNtArgs &a, const FcTnArgs &t, hipStream_t st) {
+    PSCHK(type == PS_T_F32 ? both_go<float>(a, t, st) : type == PS_T_BF16 ? both_go<__bf16>(a, t, st) : both_go<_Float16>(a, t, st));
+    return tn_reduce(t, st);
 }

@@ -54,6 +54,9 @@ struct FcTnArgs {
 };
 void fc_tn_plan(int type, FcTnArgs &a);
 int launch_fc_tn(int type, const FcTnArgs &a, hipStream_t st);
+// both products of a backward pass in one launch, where both are of few tiles
+bool fc_both_ok(int type, const FcNtArgs &a, const FcTnArgs &t);
+int launch_fc_both(int type, const FcNtArgs &a, const FcTnArgs &t, hipStream_t st);
 
 #ifdef __HIPCC__
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));

@@ -151,6 +151,7 @@ extern "C" int ps_ln_backward(ps_store_t *s, int layer, int type, const void *x_
     PSCHK(check_out(dx, sk, B, es, true));
     PSCHK(check_f32("grad_dev", grad_dev, 2ll * D, {x, dy, sk, dx}, B, es));
     PSCHK(check_f32("stats_dev", stats_dev, 2ll * B, {dx}, B, es));
+    if (grad_dev && stats_dev + 2ll * B > grad_dev && grad_dev + 2ll * D > stats_dev) return ps_set_err(PS_E_BAD_ARG, "grad_dev overlaps stats_dev");
     PSCHK(tower_enter(s));
     float *dst;
     int accum;
@@ -263,12 +264,16 @@ extern "C" int ps_fc_res_backward(ps_store_t *s, int layer, int type, int act, c
         t.D = a.A = ws + slabs;
         PSCHK(launch_act_grad(type, act, dy_dev, lddy, z_dev, ldz, ws + slabs, t.ldd, B, N, st));
     }
-    if (dx_dev) PSCHK(launch_fc_nt(type, a, ws + slabs + dzs + xs, st));
-    if (t.pack_x) {
-        PSCHK(launch_act_grad(type, PS_ACT_NONE, x_dev, ldx, nullptr, 0, ws + slabs + dzs, t.Kload, B, K, st));
-        t.X = ws + slabs + dzs; t.ldx = t.Kload;
+    if (dx_dev && fc_both_ok(type, a, t)) {
+        PSCHK(launch_fc_both(type, a, t, st));
+    } else {
+        if (dx_dev) PSCHK(launch_fc_nt(type, a, ws + slabs + dzs + xs, st));
+        if (t.pack_x) {
+            PSCHK(launch_act_grad(type, PS_ACT_NONE, x_dev, ldx, nullptr, 0, ws + slabs + dzs, t.Kload, B, K, st));
+            t.X = ws + slabs + dzs; t.ldx = t.Kload;
+        }
+        PSCHK(launch_fc_tn(type, t, st));
     }
-    PSCHK(launch_fc_tn(type, t, st));
     if (!grad_dev) p->pending_cnt++;
     return PS_OK;
 }

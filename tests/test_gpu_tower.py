@@ -627,6 +627,7 @@ def test_refusals(pool):
     assert fcb(dxp=x.p) == fcb(dxp=n.p) == N.PS_E_BAD_ARG and fcb(kp=big.p) == 0 and lnb(dxp=x.p) == N.PS_E_BAD_ARG
     assert lnb(gp=big.p) == fcb(gp=x.p) == lnf(sp=x.p) == lnb(sp=big.p) == N.PS_E_BAD_ARG
     assert lnb(gp=g.p + 1) == lnf(sp=st.p + 2) == N.PS_E_BAD_ARG
+    assert lnb(gp=st.p) == lnb(gp=st.p + 4) == N.PS_E_BAD_ARG             # the gradient over the statistics
     assert L.ps_store_create_ln(kv.h, 0, 17) == N.PS_E_STATE
     for layer, dims in ((-1, 8), (64, 8), (1, 0), (1, -3), (1, (1 << 20) + 1)):
         assert L.ps_store_create_ln(kv.h, layer, dims) == N.PS_E_BAD_ARG
