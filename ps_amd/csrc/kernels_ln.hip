@@ -378,11 +378,14 @@ int launch_ln_fwd(int type, const LnFwdArgs &a, hipStream_t st) {
     return type == PS_T_F32 ? fwd_t<float>(a, st) : type == PS_T_BF16 ? fwd_t<__bf16>(a, st) : fwd_t<_Float16>(a, st);
 }
 // Two workgroups a CU: with prefetched rows that is bytes enough in flight, and every further workgroup is a slab more to fold, write and
-// add up (bf16, 65536 x 1024: 111 us with 512 workgroups, 130 with 768, 119 with 1024, 128 with 1536; f32, 65536 x 256: 56 / 75 / 77 / 95)
+// add up (bf16, 65536 x 1024: 111 us with 512 workgroups, 130 with 768, 119 with 1024, 128 with 1536; f32, 65536 x 256: 56 / 75 / 77 / 95).
+// One a CU where the rows are few: up to 8 row groups a workgroup the slabs cost more than the rows (512 / 256: bf16, 4096 x 512 12.3 / 11.0,
+// f16, 4096 x 1024 17.9 / 14.6, f32, 8192 x 256 13.1 / 11.4, bf16, 8192 x 512 14.3 / 14.5; beyond: 16384 x 512 18.3 / 21.2, 32768 x 512
+// 25.9 / 35.8); and for rows of 512 lanes, which fill a CU by themselves.
 int ln_bwd_blocks(int type, int B, int D) {
     const Layout l = layout_of(type == PS_T_F32 ? 4 : 8, D);
     const int rpb = l.tpr && l.tpr < 256 ? 256 / l.tpr : 1;
-    const int64_t need = ((int64_t)B + rpb - 1) / rpb, most = l.tpr > 256 ? 256 : 512;
+    const int64_t need = ((int64_t)B + rpb - 1) / rpb, most = l.tpr > 256 || need <= 2048 ? 256 : 512;
     return (int)(need < most ? need : most);
 }
 int launch_ln_bwd(int type, const LnBwdArgs &a, int nblk, hipStream_t st) {
