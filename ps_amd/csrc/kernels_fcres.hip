@@ -114,9 +114,11 @@ template <typename T> __device__ __forceinline__ void load_w(Chunk<T> &o, const 
 template <typename T> struct Weights {
     f32x4 lo, hi;
     __device__ __forceinline__ void load(const float *p) { lo = reinterpret_cast<const f32x4 *>(p)[0]; hi = reinterpret_cast<const f32x4 *>(p)[1]; }
-    __device__ __forceinline__ void load(const float *row, int c, int n) {
+    // zeros behind n; the store's rows are padded to multiples of 16, so a piece that begins in one lies in it
+    __device__ __forceinline__ void load_cut(const float *row, int c, int n) {
+        load(row + (c < n ? c : 0));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { lo[j] = c + j < n ? row[c + j] : 0.f; hi[j] = c + 4 + j < n ? row[c + 4 + j] : 0.f; }
+        for (int j = 0; j < 4; ++j) { lo[j] = c + j < n ? lo[j] : 0.f; hi[j] = c + 4 + j < n ? hi[j] : 0.f; }
     }
     __device__ __forceinline__ Chunk<T> rounded() const {
         Chunk<T> o;
@@ -128,7 +130,11 @@ template <typename T> struct Weights {
 template <> struct Weights<float> {
     Chunk<float> w;
     __device__ __forceinline__ void load(const float *p) { w.u = *reinterpret_cast<const u32x4 *>(p); }
-    __device__ __forceinline__ void load(const float *row, int c, int n) { w.load(row, c, n); }
+    __device__ __forceinline__ void load_cut(const float *row, int c, int n) {
+        load(row + (c < n ? c : 0));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w.e[j] = c + j < n ? w.e[j] : 0.f;
+    }
     __device__ __forceinline__ Chunk<float> rounded() const { return w; }
 };
 
@@ -187,12 +193,12 @@ __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int t
 #pragma unroll
         for (int i = 0; i < PB; ++i) rb[set][i].load(pb[i] + k);
     };
-    auto fetch_cut = [&](int k0) {
+    auto fetch_cut = [&](int k0) {               // (a.K >= CN)
         const int k = k0 + ch * CN;
 #pragma unroll
-        for (int i = 0; i < PA; ++i) ra[0][i].load(pa[i], k, a.K);
+        for (int i = 0; i < PA; ++i) ra[0][i].load_cut(pa[i], k, a.K);
 #pragma unroll
-        for (int i = 0; i < PB; ++i) rb[0][i].load(pb[i], k, a.K);
+        for (int i = 0; i < PB; ++i) rb[0][i].load_cut(pb[i], k, a.K);
     };
     auto put = [&](int set, int buf) {
 #pragma unroll
@@ -228,7 +234,14 @@ __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int t
     const int full = a.K / BK, cut = a.K % BK ? 1 : 0, total = full + cut;
     const int lo = total * grp / G, mine = total * (grp + 1) / G - lo, steps = (total + G - 1) / G;      // (with G > 1 every group has a step)
     if (!full) {                                 // nothing but the cut step
-        fetch_cut(0);
+        if (a.K >= CN) {
+            fetch_cut(0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PA; ++i) ra[0][i].load(pa[i], ch * CN, a.K);
+#pragma unroll
+            for (int i = 0; i < PB; ++i) rb[0][i].load_cut(pb[i], ch * CN, a.K);
+        }
         put(0, 0);
         PS_WAIT_LDS(); PS_BARRIER();
         multiply(0);
@@ -361,13 +374,18 @@ __global__ __launch_bounds__(1024) void k_fc_few(FcNtArgs a, int tiles_n) {
         }
     }
     if (a.K % X::KS && full % W == wave) {
-        Chunk<T> fw, fx;
-        load_w<T>(fw, w, full * X::KS + c, a.K);
+        Chunk<T> fx[FM];
+        Weights<T> fw;
+        fw.load_cut(w, full * X::KS + c, a.K);
+        if (a.K >= Chunk<T>::N) {
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            fx.load(x[j], full * X::KS + c, a.K);
-            acc[j] = X::mma(fw, fx, acc[j]);
+            for (int j = 0; j < FM; ++j) fx[j].load_cut(x[j], full * X::KS + c, a.K);
+        } else {
+#pragma unroll
+            for (int j = 0; j < FM; ++j) fx[j].load(x[j], c, a.K);
         }
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[j] = X::mma(fw.rounded(), fx[j], acc[j]);
     }
 #pragma unroll
     for (int j = 0; j < FM; ++j) *reinterpret_cast<f32x4 *>(&sums[wave][(j * 16 + lr) * 16 + lg * 4]) = acc[j];
@@ -533,9 +551,10 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int64_t r = rx + (i & 1) * 128 + (i >> 1) * HX;
+            const T *row = A0 + (r < rows ? r : rows - 1) * a.lda;                   // (rows behind the last: their results go nowhere)
             Chunk<T> c;
-            c.zero();
-            if (r < rows) c.load(A0 + r * a.lda, steps * BIG_K + ca / 2, a.K);
+            if (a.K >= Chunk<T>::N) c.load_cut(row, steps * BIG_K + ca / 2, a.K);
+            else c.load(row, ca / 2, a.K);
             lds[steps & 1][OX[i >> 1] + (i & 1) * 512 + tid] = c.u;
         }
         PS_WAIT_LOADS(0);
@@ -609,7 +628,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T 
 // of the sum inside a step is the same for both operands and otherwise free.  32-byte pieces are exchanged by a row key: the 8 rows
 // that 32 lanes of a transposing read touch lie in different banks.  The workgroups of the first row of tiles also multiply dz by a
 // fragment of ones: db, row K of the slab.
-// Two steps ahead in registers, as in k_fc_nt: the step that M cuts off goes first and is loaded element by element.  Columns behind K and
+// Two steps ahead in registers, as in k_fc_nt: the step that M cuts off goes first, its pieces cut off in registers.  Columns behind K and
 // N are any values, their results go nowhere: whole pieces of them are read from the row's start, and a piece that the width cuts off
 // (edge) runs on into the next row -- so the step with the last row counts as cut off too.  NARROW: widths below a piece, whose pieces
 // could run past more than one row: every load element by element.
@@ -650,8 +669,15 @@ __device__ __forceinline__ void fc_tn_tile(const FcTnArgs &a, int tiles_n, int s
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int64_t m = (s_hi - 1) * ROWS + (tid + i * 256) / PER;
-            rx[0][i].zero(); rd[0][i].zero();
-            if (m < a.M) { rx[0][i].load((const T *)a.X + m * a.ldx, cx[i], a.K); rd[0][i].load((const T *)a.D + m * a.ldd, cd[i], a.N); }
+            if constexpr (NARROW) {
+                rx[0][i].zero(); rd[0][i].zero();
+                if (m < a.M) { rx[0][i].load((const T *)a.X + m * a.ldx, cx[i], a.K); rd[0][i].load((const T *)a.D + m * a.ldd, cd[i], a.N); }
+            } else {
+                const int64_t r = m < a.M ? m : a.M - 1;
+                rx[0][i].load_cut((const T *)a.X + r * a.ldx, cx[i], a.K); rd[0][i].load_cut((const T *)a.D + r * a.ldd, cd[i], a.N);
+                const u32x4 none = {0u, 0u, 0u, 0u};
+                rx[0][i].u = m < a.M ? rx[0][i].u : none; rd[0][i].u = m < a.M ? rd[0][i].u : none;
+            }
         }
     };
     auto put = [&](int set, int buf) {

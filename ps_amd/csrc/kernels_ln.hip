@@ -8,7 +8,7 @@
 // passes over them -- the variance from differences to the mean, never from sum x^2 -- and is written once; the next row's loads are in
 // flight meanwhile.  All arithmetic is f32.  A row belongs to TPR lanes (4, 16 or 64 of one wave, or a workgroup of 256 or 512) that
 // hold up to 16 elements each: a narrow row does not idle a wave, a wide one does not spill.  Rows wider than 8192 take the kernels
-// that walk the row again (from L2).  EDGE: the width is no multiple of a 16-byte piece, so the last piece is cut off element by element;
+// that walk the row again (from L2).  EDGE: the width is no multiple of a 16-byte piece, so the last piece is cut off;
 // without it a lane behind the row's end reads the row's first piece and counts it as zeros, and no load hides behind a branch.
 #include "kernels_tower.h"
 
@@ -42,15 +42,20 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float (*lds
     return s[0];
 }
 
-template <typename T, int TPR, int NV, bool EDGE> struct RowPieces {
+// CUT: the row's last piece is shifted into place without a branch, else read element by element.  It pays for the 8 elements of a 16-bit
+// piece in the forward pass (bf16, 65536 x 429: 40 us element by element, 35 shifted), not for 4 (f32, 4096 x 429: 6.8 / 7.2) nor for the
+// backward pass's three operands (bf16, 65536 x 1001: 170 / 186).
+template <typename T, int TPR, int NV, bool EDGE, bool CUT> struct RowPieces {
     static constexpr int VEC = Chunk<T>::N;
     Chunk<T> c[NV];
     __device__ __forceinline__ void load(const T *row, int t, int D) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int e = (t + i * TPR) * VEC;
-            if constexpr (EDGE) c[i].load(row, e, D);
-            else c[i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(row + (e < D ? e : 0));
+            if constexpr (EDGE) {
+                if (CUT && D >= VEC) c[i].load_cut(row, e, D);
+                else c[i].load(row, e, D);
+            } else c[i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(row + (e < D ? e : 0));
         }
     }
     __device__ __forceinline__ void store(T *row, int t, int D) const {
@@ -87,7 +92,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_fwd(LnFwdArgs a) {
     const int64_t stride = (int64_t)gridDim.x * RPB;
     int64_t r = (int64_t)blockIdx.x * RPB + sub;
     // a lane group behind the last row repeats it and writes nothing
-    RowPieces<T, TPR, NV, EDGE> v, next;
+    RowPieces<T, TPR, NV, EDGE, sizeof(T) == 2> v, next;
     next.load((const T *)a.x + (r < a.B ? r : a.B - 1) * a.ldx, t, a.D);
     float g[NV * VEC], b[NV * VEC];
     load_params<T, TPR, NV>(g, a.gamma, t, a.D);
@@ -171,7 +176,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_bwd(LnBwdArgs a) {
     const float inv_d = 1.f / (float)a.D;
     const int64_t stride = (int64_t)gridDim.x * RPB;
     int64_t r = (int64_t)blockIdx.x * RPB + sub;
-    RowPieces<T, TPR, NV, EDGE> x, dy, k, nx, ndy, nk;
+    RowPieces<T, TPR, NV, EDGE, false> x, dy, k, nx, ndy, nk;
     float mean, rstd, nmean, nrstd;
     auto fetch = [&](int64_t q) {
         if (q >= a.B) q = a.B - 1;

@@ -30,7 +30,7 @@ int launch_grad_reduce(const float *part, int nslab, int64_t n, int B, float *ds
 // Y[m][n] = act(sum_k A[m][k] * Wr[n][k] + bias[n]) + R[m][n], Z = the pre-activation; Wr f32, rounded to the activations' type on the way
 struct FcNtArgs {
     const void *A; int64_t lda;
-    const float *W; int ldw;           // [N][ldw], ldw % 4 == 0, 16-byte aligned
+    const float *W; int ldw;           // [N][ldw], rows padded to a multiple of 16, 16-byte aligned
     const float *bias;                 // [N] or NULL
     const void *R; int64_t ldr;        // NULL: none
     void *Z; int64_t ldz;              // NULL: none
@@ -90,8 +90,20 @@ template <typename T> struct Chunk {
         for (int j = 0; j < N; ++j)
             if (c + j < n) e[j] = row[c + j];
     }
+    // the same without a branch, for n >= N: the piece that the row's end cuts off is read further to the left and shifted down (a load
+    // behind a branch waits by itself, and these are often a call's first)
+    __device__ __forceinline__ void load_cut(const T *row, int c, int n) {
+        const int at = c < n - N ? c : n - N, s = c - at;
+        u = *reinterpret_cast<const unaligned_t *>(row + at);
+        constexpr int ODD = sizeof(T) == 2 ? 1 : 0;                          // elements to a word: 2 or 1
+        if constexpr (ODD)
+            u = s & 1 ? u32x4{__builtin_amdgcn_alignbit(u[1], u[0], 16), __builtin_amdgcn_alignbit(u[2], u[1], 16), __builtin_amdgcn_alignbit(u[3], u[2], 16), u[3] >> 16} : u;
+        u = (s >> ODD) & 1 ? u32x4{u[1], u[2], u[3], 0u} : u;
+        u = (s >> ODD) & 2 ? u32x4{u[2], u[3], 0u, 0u} : u;
+        u = s >= N ? u32x4{0u, 0u, 0u, 0u} : u;
+    }
     __device__ __forceinline__ void store(T *row, int c, int n) const {
-                if (c + N <= n) { *reinterpret_cast<unaligned_t *>(row + c) = u; return; }
+        if (c + N <= n) { *reinterpret_cast<unaligned_t *>(row + c) = u; return; }
 #pragma unroll
         for (int j = 0; j < N; ++j)
             if (c + j < n) row[c + j] = e[j];
