@@ -31,58 +31,49 @@ template <> struct Mma<float> {        // a fragment holds 4 steps of 2: the lan
     }
 };
 
-// The normal law's tail Q(|z|) = erfc(|z| / sqrt 2) / 2 and density: Abramowitz & Stegun 7.1.26 (|error of erfc| < 1.5e-7: about the
-// rounding of 1 + erf in f32), whose e^(-z^2 / 2) the slope needs anyway.  About 20 instruction slots with one reciprocal and one
-// exponential, a third of the library's erff.
-__device__ __forceinline__ float normal_tail(float z, float &e) {
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
-    e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);                       // e^(-z^2 / 2)
-    float p = fmaf(1.061405429f, t, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    return 0.5f * p * t * e;
-}
-__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
-// Q(|z|) alone: 2 to a polynomial of |z| for log2 Q, which is nearly a parabola -- a least maximum of |error of Q| / (Q + 0.01) on
-// [0, 5.5], falling from there on.  |error| < 8e-8, relative below 2e-5 up to 4 and 3e-3 at 5: what 16 bits can tell, and 13 slots; in the
-// epilogue of a product nothing hides them.
-__device__ __forceinline__ float normal_tail_16(float z) {
+// The normal law's tail Q(|z|) = erfc(|z| / sqrt 2) / 2 as 2 to a polynomial of |z|: log2 Q is nearly a parabola, and the polynomial is the
+// one of degree 8 whose greatest |error of Q| on [0, 6] is least; it falls from there on.  |error| < 4e-8, the rounding of numbers
+// near 1/2 (relative below 2e-6 up to 3, 2e-4 at 4), from 8 multiply-adds and one exponential: in the epilogue of a product nothing
+// hides them.
+__device__ __forceinline__ float normal_tail(float z) {
     const float x = fabsf(z);
-    float p = fmaf(-1.62304002e-6f, x, 2.44227995e-5f);
-    p = fmaf(p, x, -1.12760834e-4f);
-    p = fmaf(p, x, -3.20743507e-4f);
-    p = fmaf(p, x, 7.31313042e-3f);
-    p = fmaf(p, x, -0.0526767336f);
-    p = fmaf(p, x, -0.459145278f);
-    p = fmaf(p, x, -1.15111339f);
-    return __builtin_amdgcn_exp2f(fmaf(p, x, -0.999999821f));
+    float p = fmaf(-2.77219374e-6f, x, 3.86222273e-5f);
+    p = fmaf(p, x, -1.82553558e-4f);
+    p = fmaf(p, x, -1.45858037e-4f);
+    p = fmaf(p, x, 7.07545876e-3f);
+    p = fmaf(p, x, -0.0525050201f);
+    p = fmaf(p, x, -0.459204912f);
+    p = fmaf(p, x, -1.15110576f);
+    return __builtin_amdgcn_exp2f(fmaf(p, x, -1.f));
 }
-template <typename T, int NV> __device__ __forceinline__ void act_apply(float (&v)[NV], int act) {
+template <int NV> __device__ __forceinline__ void act_apply(float (&v)[NV], int act) {
     if (act == PS_ACT_RELU) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];        // (a NaN stays one)
     } else if (act == PS_ACT_GELU) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {           // z Phi(z) = max(z, 0) - |z| Q(|z|), and Q(64) is 0 (so is Q(infinity) times it)
-            float e, q;
-            if constexpr (sizeof(T) == 2) q = normal_tail_16(v[j]); else q = normal_tail(v[j], e);
-            v[j] = fmaf(-fminf(fabsf(v[j]), 64.f), q, fmaxf(v[j], 0.f));
-        }
+        for (int j = 0; j < NV; ++j)             // z Phi(z) = max(z, 0) - |z| Q(|z|), and Q(64) is 0 (so is Q(infinity) times it)
+            v[j] = fmaf(-fminf(fabsf(v[j]), 64.f), normal_tail(v[j]), fmaxf(v[j], 0.f));
     } else if (act == PS_ACT_SILU) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] *= logistic(v[j]);
+        for (int j = 0; j < NV; ++j) v[j] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v[j]));
     }
 }
+// GELU' = Phi(z) + z phi(z); SILU' = s (1 + z (1 - s)) with s = 1 / (1 + e^-z), from e^-|z|, which does not overflow.  As exact as f32
+// formulas with a library's erf and exp are (mean |error| over normal z 2.3e-8 and 2.0e-8; those have 2.0e-8 and 2.1e-8): dz is rounded to
+// 16 bits, and every value that a slope's error sends to the other neighbour is a whole step in dW's sums -- with an error of 1e-7 dW's was
+// 1.7 times as large.  The pass is bound by memory and does not notice.
 __device__ __forceinline__ float act_slope(float z, int act) {
-    const float x = fminf(fmaxf(z, -128.f), 128.f);      // (beyond, both slopes are 0 and 1 to the last bit, and infinity times 0 is not)
+    const float x = fabsf(z) > 128.f ? 128.f : fabsf(z); // (beyond, both slopes are 0 and 1 to the last bit, and infinity times 0 is not)
     if (act == PS_ACT_GELU) {
-        float e;
-        const float q = normal_tail(z, e);
-        return fmaf(x * 0.39894228f, e, z < 0.f ? q : 1.f - q);
+        const float q = normal_tail(z), d = x * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+        return z < 0.f ? q - d : 1.f - (q - d);
     }
-    const float p = logistic(z);
-    return p * fmaf(x, 1.f - p, 1.f);
+    const float e = __builtin_amdgcn_exp2f(-1.44269504f * x), d = 1.f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.f), r, r);
+    const float q = z < 0.f ? e * r : r;
+    return q * fmaf(z < 0.f ? -x : x, 1.f - q, 1.f);
 }
 
 // workgroup -> tile so that an XCD (workgroup id mod 8) owns a contiguous range of tiles: its L2 then serves the tiles' shared rows
@@ -308,7 +299,7 @@ __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int t
                     for (int e = 0; e < 4; ++e) o.e[e] = (T)v[e];
                     o.store(zr, n, a.N);
                 }
-                act_apply<T>(v, a.act);
+                act_apply(v, a.act);
                 if (a.R) {
                     o.load(rr, n, a.N);
 #pragma unroll
@@ -398,7 +389,7 @@ __global__ __launch_bounds__(1024) void k_fc_few(FcNtArgs a, int tiles_n) {
     for (int q = 0; q < W; ++q) v[0] += sums[q][threadIdx.x];
     if (a.bias) v[0] += a.bias[n];
     if (a.Z) ((T *)a.Z)[m * a.ldz + n] = (T)v[0];
-    act_apply<T>(v, a.act);
+    act_apply(v, a.act);
     if (a.R) v[0] += (float)((const T *)a.R)[m * a.ldr + n];
     ((T *)a.Y)[m * a.ldy + n] = (T)v[0];
 }
@@ -585,7 +576,7 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
                 o.store((T *)a.Z + m * a.ldz, n + h * 8, a.N);
             }
         }
-        act_apply<T>(v, a.act);
+        act_apply(v, a.act);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (a.R) {
