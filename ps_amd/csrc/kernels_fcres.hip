@@ -59,21 +59,24 @@ template <int NV> __device__ __forceinline__ void act_apply(float (&v)[NV], int 
         for (int j = 0; j < NV; ++j) v[j] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v[j]));
     }
 }
-// GELU' = Phi(z) + z phi(z); SILU' = s (1 + z (1 - s)) with s = 1 / (1 + e^-z), from e^-|z|, which does not overflow.  As exact as f32
-// formulas with a library's erf and exp are (mean |error| over normal z 2.3e-8 and 2.0e-8; those have 2.0e-8 and 2.1e-8): dz is rounded to
-// 16 bits, and every value that a slope's error sends to the other neighbour is a whole step in dW's sums -- with an error of 1e-7 dW's was
-// 1.7 times as large.  The pass is bound by memory and does not notice.
-__device__ __forceinline__ float act_slope(float z, int act) {
-    const float x = fabsf(z) > 128.f ? 128.f : fabsf(z); // (beyond, both slopes are 0 and 1 to the last bit, and infinity times 0 is not)
+// dy times GELU' = Phi(z) + z phi(z) or SILU' = s (1 + z (1 - s)), s = 1 / (1 + e^-z).  Both slopes are w(|z|) below 0 and 1 - w(|z|) above:
+// the 1 goes into the product's own rounding.  dz is rounded to 16 bits, and every value that a slope's error sends to the other
+// neighbour is a whole step in dW's sums.  (With a slope 1e-7 off, dW of 32768 x 1024 -> 4096 with GELU was 6.3e-6 off; so 0.6e-6, where
+// f32 formulas with a library's erf leave 3.7e-6.)  The pass is bound by memory and does not notice.
+__device__ __forceinline__ float act_grad(float dy, float z, int act) {
+    const float x = fabsf(z) > 128.f ? 128.f : fabsf(z); // (beyond, w is 0 to the last bit, and infinity times 0 is not)
+    float w;
     if (act == PS_ACT_GELU) {
-        const float q = normal_tail(z), d = x * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * z * z);
-        return z < 0.f ? q - d : 1.f - (q - d);
+        w = fmaf(x * -0.39894228f, __builtin_amdgcn_exp2f(-0.72134752f * z * z), normal_tail(z));
+    } else {
+        // e^-x as 2^t (1 + what t's rounding and log2 e's leave), 1 / (1 + e) as r + c, so that 1 - x / (1 + e) is exact at its zero
+        const float t = -1.44269504f * x, p = __builtin_amdgcn_exp2f(t);
+        const float e = fmaf(p, 0.69314718f * fmaf(-1.92596299e-8f, x, fmaf(-1.44269504f, x, -t)), p), d = 1.f + e;
+        const float r = __builtin_amdgcn_rcpf(d), c = r * fmaf(-r, e - (d - 1.f), fmaf(-d, r, 1.f));
+        w = e * (r + c) * fmaf(-x, c, fmaf(-x, r, 1.f));
     }
-    const float e = __builtin_amdgcn_exp2f(-1.44269504f * x), d = 1.f + e;
-    float r = __builtin_amdgcn_rcpf(d);
-    r = fmaf(fmaf(-d, r, 1.f), r, r);
-    const float q = z < 0.f ? e * r : r;
-    return q * fmaf(z < 0.f ? -x : x, 1.f - q, 1.f);
+    const float dz = z < 0.f ? dy * w : fmaf(-dy, w, dy);
+    return dz == dz ? dz : dy * (z < 0.f ? w : 1.f - w);                     // (an infinite dy is one behind a slope, too)
 }
 
 // workgroup -> tile so that an XCD (workgroup id mod 8) owns a contiguous range of tiles: its L2 then serves the tiles' shared rows
@@ -606,7 +609,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T 
 #pragma unroll
                 for (int j = 0; j < Chunk<T>::N; ++j) {
                     const float zz = (float)v.e[j];
-                    d.e[j] = act == PS_ACT_RELU ? (zz > 0.f ? d.e[j] : (T)0.f) : (T)((float)d.e[j] * act_slope(zz, act));
+                    d.e[j] = act == PS_ACT_RELU ? (zz > 0.f ? d.e[j] : (T)0.f) : (T)act_grad((float)d.e[j], zz, act);
                 }
             }
         }
