@@ -152,6 +152,9 @@ template <> struct Weights<float> {
 // G > 1: the groups share the sum out -- for outputs of few tiles, whose chain of steps is what a call costs -- and add up through LDS, in
 // group order.
 // The product is formed transposed (weights as the first operand): a lane then holds 4 neighbouring columns of one row of y.
+// Measured: f32, 4096 x 429 -> 512, relu, z kept 22 us (82 TF; matrix units busy 0.63 of the launch, the rest is its start, first loads
+// and end; the order and number of accumulators makes no difference), 8192 x 2048 -> 2048 567 us (121 TF, 0.82 of a library's bare
+// product); bf16, 4096 x 429 -> 512 10 us.
 template <typename T, int BM, int BN, int AHEAD, int G>
 __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int tile, u32x4 *lds) {
     typedef Mma<T> X;
@@ -159,8 +162,10 @@ __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int t
     constexpr int CN = Chunk<T>::N, BK = X::BK, TILE = X::TILE, FM = BM / 2 / TILE, FN = BN / 2 / TILE, PA = BM * 8 / 256, PB = BN * 8 / 256;
     const int64_t m0 = (int64_t)(tile / tiles_n) * BM;
     const int n0 = (tile % tiles_n) * BN;
-    const int tid = threadIdx.x & 255, grp = G > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-    u32x4(*sA)[BM * 8] = reinterpret_cast<u32x4(*)[BM * 8]>(lds + grp * 2 * (BM + BN) * 8), (*sB)[BN * 8] = reinterpret_cast<u32x4(*)[BN * 8]>(lds + grp * 2 * (BM + BN) * 8 + 2 * BM * 8);
+    const int tid = threadIdx.x & 255, grp = G > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0, lane = tid & 63, wave = tid >> 6;
+    const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+    u32x4 *own = lds + grp * 2 * (BM + BN) * 8;
+    u32x4(*sA)[BM * 8] = reinterpret_cast<u32x4(*)[BM * 8]>(own), (*sB)[BN * 8] = reinterpret_cast<u32x4(*)[BN * 8]>(own + 2 * BM * 8);
     const T *pa[PA];
     const float *pb[PB];
     int dst_a[PA], dst_b[PB];
@@ -323,6 +328,7 @@ __global__ __launch_bounds__(256 * G, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a,
 // Few rows (or few tiles): one workgroup of 16 waves per 16 columns and 16 FM rows.  The waves share out the sum in steps and take their
 // fragments straight from memory -- the weights in f32, rounded in registers, each read once per row of tiles -- so that a call is two
 // dependent trips to memory and not a chain of staged steps; their sums meet in LDS and are added in wave order.
+// Bound by latency: 3.4 us on the device for one row of 429 -> 512, 6.8 us for bf16, 16 x 2048 -> 2048 (16.8 MB of weights, 2.5 TB/s).
 template <typename T> struct MmaFew {
     static constexpr int KS = 32;
     static __device__ __forceinline__ f32x4 mma(const Chunk<T> &a, const Chunk<T> &b, f32x4 c) {
@@ -397,7 +403,8 @@ __global__ __launch_bounds__(1024) void k_fc_few(FcNtArgs a, int tiles_n) {
     ((T *)a.Y)[m * a.ldy + n] = (T)v[0];
 }
 
-// The weights of a product in the activations' type, laid out for k_fc_nt_big: rows padded with zeros to a multiple of BK and of BN
+// The weights of a product in the activations' type, laid out for k_fc_nt_big: rows padded with zeros to a multiple of BK and of BN.  In
+// every call -- a copy kept from one call to the next would have to learn of every update: 6 to 8 us for 4.2 M weights (3.5 TB/s).
 template <typename T> __global__ __launch_bounds__(256) void k_cast_w(const float *__restrict__ W, int ldw, int N, int K, T *__restrict__ out, int Kp, int Np) {
     const int per = Kp / 8;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -431,6 +438,10 @@ typedef __attribute__((address_space(3))) void lds_void;
 // faster than 64 bytes of four lanes per store).
 // Rows of x behind the last read as zeros through the buffer's bound; a last step that K does not fill goes through registers, where
 // its tail is cut off.
+// Measured: bf16, 8192 x 8192 -> 8192 1320 TF, 32768 x 4096 -> 1024 1190 (a library's bare products 1330 and 1240): the clock that the power
+// limit leaves bounds these.  32768 x 1024 -> 4096 with GELU and z kept 319 us (860 TF): 16 steps of 64 are 20 us of a tile's 38, its first
+// loads, GELU's arithmetic and the stores the rest, and nothing overlaps them: two workgroups a CU of 256 x 128 tiles in steps of 32 do,
+// but their loop runs at 990 TF where this one has 1320, and lose (377 us).
 template <typename T, int BN>
 __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, int Kp, int tiles_m, int tiles_n) {
     typedef Mma<T> X;
@@ -594,7 +605,9 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
     }
 }
 
-// dz = dy act'(z), rounded to the type; z NULL: a copy.  dz's rows are 16-byte pieces, zeros behind the width.
+// dz = dy act'(z), rounded to the type; z NULL: a copy.  dz's rows are 16-byte pieces, zeros behind the width.  Bound by memory: bf16,
+// 32768 x 4096 148 us, 5.4 TB/s.  (dz is read by both products of the pass, many times over: forming it on the way into each of them
+// would cost its arithmetic once per tile.)
 template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T *dy, int64_t lddy, const T *z, int64_t ldz, T *dz, int64_t lddz, int M, int N, int act) {
     const int64_t per = lddz / Chunk<T>::N, total = per * M;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -795,6 +808,7 @@ __global__ __launch_bounds__(256, BT == 64 ? 3 : 2) void k_fc_tn(FcTnArgs a, int
     __shared__ u32x4 lds[kTnLds<T, BT>];
     fc_tn_part<T, BT>(a, tiles_n, tiles, xcd_tile(blockIdx.x, gridDim.x), lds);
 }
+// Measured (k_fc_tn with k_fc_grad_reduce): f32, 8192 x 1024 -> 1024, both gradients 313 us (110 TF).
 // dW's tiles and, behind them, dx's, in one launch: where neither fills the chip they run side by side, and there is one start and one end
 // less (two launches / one: bf16, 4096 x 512 -> 256 with relu 24.7 / 21.5 us, 4096 x 429 -> 512 with GELU 30.2 / 25.4; f32 40.8 / 35.4 and
 // 57.2 / 52.0; where the chip is full no difference: f32, 16384 x 429 -> 512 169.7 / 168.2, bf16, 100000 x 64 -> 64 38.2 / 38.5).
@@ -821,6 +835,7 @@ __device__ __forceinline__ s16x4 read_transposed(const short *__restrict__ p) {
 // db is dz times a fragment of ones: every workgroup of a row of tiles, and of it one of the two wave rows, takes its share of the
 // steps, so that no workgroup is the slow one; each leaves its own row behind dW's in the slab.
 // Columns behind K and N, and rows behind the part's last, are sent out of the buffer's bounds: zeros.
+// Measured: bf16, 32768 x 1024 -> 4096 248 us with its reduction (1107 TF; a library's bare product 346 us), matrix units busy 0.63, LDS 0.23.
 template <typename T>
 __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, int tiles_n) {
     typedef Mma<T> X;
@@ -979,8 +994,8 @@ __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, i
 }
 
 // The slabs' sum and mean: dW over the parts, db over the parts and their rows.  A wave takes 256 neighbouring elements (4 a lane) and 8
-// slabs at a time.  W = 1: every wave its own elements; W = 16, many slabs: the waves of a workgroup share them out and are added in
-// wave order.  The workgroups behind dW's do db, 64 columns each.
+// slabs at a time: 15 us for 4 slabs of 1024 x 4096 (5.6 TB/s, from the Infinity Cache).  W = 1: every wave its own elements; W = 16,
+// many slabs: the waves of a workgroup share them out and are added in wave order.  The workgroups behind dW's do db, 64 columns each.
 template <int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 1024) void k_fc_grad_reduce(FcTnArgs a, int dw_blocks) {
     typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
