@@ -213,6 +213,16 @@ __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int t
 #pragma unroll
             for (int e = 0; e < (int)(sizeof(acc[0][0]) / 4); ++e) acc[i][j][e] = 0.f;
     const int lr = lane % TILE, lg = lane / TILE;
+    constexpr int GR = (int)(sizeof(acc[0][0]) / 16);            // a lane's results: GR groups of 4 neighbouring columns of one row
+    f32x4 bias[FN][GR];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int q = 0; q < GR; ++q) {
+            const int n = n0 + wn + i * TILE + q * 8 + lg * 4;
+            bias[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (a.bias) bias[i][q] = *reinterpret_cast<const f32x4 *>(a.bias + (n < a.N ? n : 0));      // (its row is padded to a multiple of 16)
+        }
     constexpr int KS = 8 / (64 / TILE);          // fragment steps per LDS row
     auto multiply = [&](int buf) {
 #pragma unroll
@@ -284,14 +294,28 @@ __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int t
 #pragma unroll
                     for (int e = 0; e < AE; ++e) acc[i][j][e] += sums[((g * FN + i) * FM + j) * AE * 256 + e * 256];
     }
-    // epilogue: groups of 4 neighbouring columns of one row
-    constexpr int GR = (int)(sizeof(acc[0][0]) / 16);
+    // epilogue: the residual first -- a load behind a store waits for the store, too
+    Quad<T> res[FM][FN][GR];
+    if (a.R) {
+        const bool whole = n0 + BN <= a.N;
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            const int64_t m = m0 + wm + j * TILE + lr;
+            const T *rr = (const T *)a.R + (m < a.M ? m : a.M - 1) * a.ldr;
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int q = 0; q < GR; ++q) {
+                    const int n = n0 + wn + i * TILE + q * 8 + lg * 4;
+                    if (whole) res[j][i][q].load(rr + n); else res[j][i][q].load(rr, n, a.N);
+                }
+        }
+    }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
         const int64_t m = m0 + wm + j * TILE + lr;
         if (m >= a.M) continue;
         T *y = (T *)a.Y + m * a.ldy, *zr = (T *)a.Z + m * a.ldz;
-        const T *rr = (const T *)a.R + m * a.ldr;
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
@@ -301,18 +325,16 @@ __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int t
                 float v[4];
                 Quad<T> o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e] + (a.bias ? a.bias[n + e] : 0.f);      // (the bias row is padded to a multiple of 16)
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e] + bias[i][q][e];
                 if (a.Z) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o.e[e] = (T)v[e];
                     o.store(zr, n, a.N);
                 }
                 act_apply(v, a.act);
-                if (a.R) {
-                    o.load(rr, n, a.N);
+                if (a.R)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += (float)o.e[e];
-                }
+                    for (int e = 0; e < 4; ++e) v[e] += (float)res[j][i][q].e[e];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o.e[e] = (T)v[e];
                 o.store(y, n, a.N);
@@ -359,6 +381,14 @@ __global__ __launch_bounds__(1024) void k_fc_few(FcNtArgs a, int tiles_n) {
         const int64_t m = m0 + j * 16 + lr;
         x[j] = (const T *)a.A + (m < a.M ? m : a.M - 1) * a.lda;
     }
+    // the thread's result, and what is added to it: asked for first, there when the sums are
+    const int64_t m = m0 + (threadIdx.x >> 4);
+    const int n = n0 + (threadIdx.x & 15);
+    const bool mine = (int)threadIdx.x < FM * 256 && m < a.M && n < a.N;
+    float bias = 0.f;
+    T res = (T)0.f;
+    if (mine && a.bias) bias = a.bias[n];
+    if (mine && a.R) res = ((const T *)a.R)[m * a.ldr + n];
     f32x4 acc[FM];
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -390,16 +420,14 @@ __global__ __launch_bounds__(1024) void k_fc_few(FcNtArgs a, int tiles_n) {
 #pragma unroll
     for (int j = 0; j < FM; ++j) *reinterpret_cast<f32x4 *>(&sums[wave][(j * 16 + lr) * 16 + lg * 4]) = acc[j];
     __syncthreads();
-    const int64_t m = m0 + (threadIdx.x >> 4);
-    const int n = n0 + (threadIdx.x & 15);
-    if ((int)threadIdx.x >= FM * 256 || m >= a.M || n >= a.N) return;
+    if (!mine) return;
     float v[1] = {0.f};
 #pragma unroll
     for (int q = 0; q < W; ++q) v[0] += sums[q][threadIdx.x];
-    if (a.bias) v[0] += a.bias[n];
+    v[0] += bias;
     if (a.Z) ((T *)a.Z)[m * a.ldz + n] = (T)v[0];
     act_apply(v, a.act);
-    if (a.R) v[0] += (float)((const T *)a.R)[m * a.ldr + n];
+    if (a.R) v[0] += (float)res;
     ((T *)a.Y)[m * a.ldy + n] = (T)v[0];
 }
 
@@ -540,6 +568,13 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
         ask_w(t + 2, 1);
         PS_WAIT_LOADS(2 * LX + 3 * LW); turn(); multiply(1, 0); turn();
     }
+    const int n = n0 + wn * 64 + lg * 16;
+    f32x4 bias[4];                               // (its row is padded to a multiple of 16)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bias[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (a.bias) bias[e] = reinterpret_cast<const f32x4 *>(a.bias + (n < a.N ? n : 0))[e];
+    }
     for (; t < steps; ++t) {                     // the last two: nothing but x1 is left to ask for
         read_x(t, 0); read_w(t, 0);
         if (t + 1 < steps) ask_x(t + 1, 1);
@@ -569,11 +604,22 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
         read_x(steps, 1);
         multiply(1, 1); multiply(1, 0);
     }
-    const int n = n0 + wn * 64 + lg * 16;
     if (n >= a.N) return;
-    float bias[16];
+    Chunk<T> res[2 * FJ][2];                     // the residual first: a load behind a store waits for the store, too
+    if (a.R) {
+        const bool whole = n0 + BN <= a.N;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) bias[e] = a.bias ? a.bias[n + e] : 0.f;      // (the bias row is padded to a multiple of 16)
+        for (int j = 0; j < 2 * FJ; ++j) {
+            const int64_t m = m0 + wm * 2 * HX + j * 16 + lr;
+            const T *row = (const T *)a.R + (m < a.M ? m : a.M - 1) * a.ldr;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (whole) res[j][h].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(row + n + h * 8);
+                else if (a.N >= Chunk<T>::N) res[j][h].load_cut(row, n + h * 8, a.N);
+                else res[j][h].load(row, n + h * 8, a.N);
+            }
+        }
+    }
 #pragma unroll
     for (int j = 0; j < 2 * FJ; ++j) {
         const int64_t m = m0 + wm * 2 * HX + j * 16 + lr;
@@ -581,7 +627,7 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
         float v[16];
         Chunk<T> o;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = acc[e >> 2][j][e & 3] + bias[e];
+        for (int e = 0; e < 16; ++e) v[e] = acc[e >> 2][j][e & 3] + bias[e >> 2][e & 3];
         if (a.Z) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -593,11 +639,9 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
         act_apply(v, a.act);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (a.R) {
-                o.load((const T *)a.R + m * a.ldr, n + h * 8, a.N);
+            if (a.R)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[h * 8 + e] += (float)o.e[e];
-            }
+                for (int e = 0; e < 8; ++e) v[h * 8 + e] += (float)res[j][h].e[e];
 #pragma unroll
             for (int e = 0; e < 8; ++e) o.e[e] = (T)v[h * 8 + e];
             o.store((T *)a.Y + m * a.ldy, n + h * 8, a.N);

@@ -113,6 +113,7 @@ template <typename T> struct Chunk {
 template <typename T> struct Quad {
     typedef typename AtElem4<(int)sizeof(T)>::v bits_t;
     T e[4];
+    __device__ __forceinline__ void load(const T *p) { const bits_t b = *reinterpret_cast<const bits_t *>(p); __builtin_memcpy(e, &b, 4 * sizeof(T)); }
     __device__ __forceinline__ void load(const T *row, int c, int n) {
         if (c + 4 <= n) { const bits_t b = *reinterpret_cast<const bits_t *>(row + c); __builtin_memcpy(e, &b, 4 * sizeof(T)); return; }
 #pragma unroll
