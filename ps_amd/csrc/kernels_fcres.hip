@@ -1038,15 +1038,15 @@ __global__ __launch_bounds__(512, 2) void k_fc_tn_big(FcTnArgs a, int tiles_k, i
 }
 
 // The slabs' sum and mean: dW over the parts, db over the parts and their rows.  A wave takes 256 neighbouring elements (4 a lane) and 8
-// slabs at a time: 15 us for 4 slabs of 1024 x 4096 (5.6 TB/s, from the Infinity Cache).  W = 1: every wave its own elements; W = 16,
-// many slabs: the waves of a workgroup share them out and are added in wave order.  The workgroups behind dW's do db, 64 columns each.
+// slabs at a time: 15 us for 4 slabs of 1024 x 4096 (5.6 TB/s, from the Infinity Cache).  W = 1: every wave its own elements; W = 4
+// and 16, many slabs: the waves of a workgroup share them out and are added in wave order.  The workgroups behind dW's do db, 64 columns each.
 template <int W>
-__global__ __launch_bounds__(W == 1 ? 256 : 1024) void k_fc_grad_reduce(FcTnArgs a, int dw_blocks) {
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_fc_grad_reduce(FcTnArgs a, int dw_blocks) {
     typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
-    __shared__ f32x4 sums[W == 1 ? 4 : 16][64];
+    __shared__ f32x4 sums[W == 1 ? 4 : W][64];
     const int64_t n = (int64_t)a.K * a.N, slab = (int64_t)(a.K + a.nbias) * a.N;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int WAVES = W == 1 ? 4 : 16;
+    constexpr int WAVES = W == 1 ? 4 : W;
     auto finish = [&](int64_t i, float s) { s /= (float)a.M; a.dst[i] = a.accum ? a.dst[i] + s : s; };
     if ((int)blockIdx.x < dw_blocks) {
         const int64_t i = (W == 1 ? ((int64_t)blockIdx.x * 4 + wave) : (int64_t)blockIdx.x) * 256 + lane * 4;
@@ -1244,9 +1244,12 @@ int tn_reduce(const FcTnArgs &a, hipStream_t st) {
     const int64_t n = (int64_t)a.K * a.N;
     const int db = cdiv(a.N, 64);
     if (a.nsplit >= 16 && n < 256 * 1024) {                  // (from one workgroup of four waves for each CU on they need not share)
+        // up to 32 slabs are one trip of four waves (16 slabs, 512 x 256: the whole pass 19.3 us, 22.3 by sixteen), more want sixteen
+        // (390 slabs, 64 x 64: 40.2 / 37.2)
         const int64_t dw = (n + 255) / 256;
         PSCHK(grid_ok(4 * (dw + db)));
-        hipLaunchKernelGGL(k_fc_grad_reduce<16>, dim3((unsigned)(dw + db)), dim3(1024), 0, st, a, (int)dw);
+        if (a.nsplit <= 32) hipLaunchKernelGGL(k_fc_grad_reduce<4>, dim3((unsigned)(dw + db)), dim3(256), 0, st, a, (int)dw);
+        else hipLaunchKernelGGL(k_fc_grad_reduce<16>, dim3((unsigned)(dw + db)), dim3(1024), 0, st, a, (int)dw);
     } else {
         const int64_t dw = (n + 1023) / 1024;
         PSCHK(grid_ok(dw + db));
