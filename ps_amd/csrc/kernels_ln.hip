@@ -44,20 +44,27 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float (*lds
     return s[0];
 }
 
-// CUT: the row's last piece is shifted into place without a branch, else read element by element.  It pays for the 8 elements of a 16-bit
-// piece in the forward pass (bf16, 65536 x 429: 40 us element by element, 35 shifted), not for 4 (f32, 4096 x 429: 6.8 / 7.2) nor for the
-// backward pass's three operands (bf16, 65536 x 1001: 170 / 186).
-template <typename T, int TPR, int NV, bool EDGE, bool CUT> struct RowPieces {
+// EDGE: the piece that the width cuts off runs on into the next row -- what it finds there is masked -- except in the last row, which reads
+// it further to the left and shifts it into place before its use (settle): no load hides behind a branch, and no other row pays.  (Shifted
+// in every row: bf16, 65536 x 1001 backward 180 us; element by element 156.)
+template <typename T, int TPR, int NV, bool EDGE> struct RowPieces {
     static constexpr int VEC = Chunk<T>::N;
     Chunk<T> c[NV];
-    __device__ __forceinline__ void load(const T *row, int t, int D) {
+    __device__ __forceinline__ void load(const T *row, int t, int D, bool last) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int e = (t + i * TPR) * VEC;
-            if constexpr (EDGE) {
-                if (CUT && D >= VEC) c[i].load_cut(row, e, D);
-                else c[i].load(row, e, D);
-            } else c[i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(row + (e < D ? e : 0));
+            if (EDGE && D < VEC) { c[i].load(row, e, D); continue; }         // (narrower than a piece: it could run past more than one row)
+            int at = e < D ? e : 0;
+            if (EDGE && last && at + VEC > D) at = D - VEC;
+            c[i].u = *reinterpret_cast<const typename Chunk<T>::unaligned_t *>(row + at);
+        }
+    }
+    __device__ __forceinline__ void settle(int t, int D) {                   // of the last row
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = (t + i * TPR) * VEC;
+            if (D >= VEC && e < D && e + VEC > D) c[i].shift_down(e + VEC - D);
         }
     }
     __device__ __forceinline__ void store(T *row, int t, int D) const {
@@ -99,14 +106,15 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_fwd(LnFwdArgs a) {
     const int64_t stride = (int64_t)gridDim.x * RPB;
     int64_t r = (int64_t)blockIdx.x * RPB + sub;
     // a lane group behind the last row repeats it and writes nothing
-    RowPieces<T, TPR, NV, EDGE, sizeof(T) == 2> v, next;
-    next.load((const T *)a.x + (r < a.B ? r : a.B - 1) * a.ldx, t, a.D);
+    RowPieces<T, TPR, NV, EDGE> v, next;
+    next.load((const T *)a.x + (r < a.B ? r : a.B - 1) * a.ldx, t, a.D, r >= a.B - 1);
     float g[NV * VEC], b[NV * VEC];
     load_params<T, TPR, NV, EDGE>(g, a.gamma, t, a.D);
     load_params<T, TPR, NV, EDGE>(b, a.beta, t, a.D);
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.B; r0 += stride, r += stride) {
         v = next;
-        if (r0 + stride < a.B) next.load((const T *)a.x + (r + stride < a.B ? r + stride : a.B - 1) * a.ldx, t, a.D);
+        if (EDGE && r >= a.B - 1) v.settle(t, a.D);
+        if (r0 + stride < a.B) next.load((const T *)a.x + (r + stride < a.B ? r + stride : a.B - 1) * a.ldx, t, a.D, r + stride >= a.B - 1);
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -183,13 +191,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_bwd(LnBwdArgs a) {
     const float inv_d = 1.f / (float)a.D;
     const int64_t stride = (int64_t)gridDim.x * RPB;
     int64_t r = (int64_t)blockIdx.x * RPB + sub;
-    RowPieces<T, TPR, NV, EDGE, false> x, dy, k, nx, ndy, nk;
+    RowPieces<T, TPR, NV, EDGE> x, dy, k, nx, ndy, nk;
     float mean, rstd, nmean, nrstd;
     auto fetch = [&](int64_t q) {
-        if (q >= a.B) q = a.B - 1;
-        nx.load((const T *)a.x + q * a.ldx, t, a.D);
-        ndy.load((const T *)a.dy + q * a.lddy, t, a.D);
-        if (a.skip) nk.load((const T *)a.skip + q * a.ldskip, t, a.D);
+        const bool last = q >= a.B - 1;
+        if (last) q = a.B - 1;
+        nx.load((const T *)a.x + q * a.ldx, t, a.D, last);
+        ndy.load((const T *)a.dy + q * a.lddy, t, a.D, last);
+        if (a.skip) nk.load((const T *)a.skip + q * a.ldskip, t, a.D, last);
         nmean = a.stats[2 * q]; nrstd = a.stats[2 * q + 1];
     };
 #pragma unroll
@@ -202,6 +211,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_bwd(LnBwdArgs a) {
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.B; r0 += stride, r += stride) {
         const bool live = r < a.B;
         x = nx; dy = ndy; k = nk; mean = nmean; rstd = nrstd;
+        if (EDGE && r >= a.B - 1) {
+            x.settle(t, a.D); dy.settle(t, a.D);
+            if (a.skip) k.settle(t, a.D);
+        }
         if (r0 + stride < a.B) fetch(r + stride);
         float s[2] = {0.f, 0.f};
 #pragma unroll

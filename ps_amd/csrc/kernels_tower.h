@@ -93,9 +93,13 @@ template <typename T> struct Chunk {
     // the same without a branch, for n >= N: the piece that the row's end cuts off is read further to the left and shifted down (a load
     // behind a branch waits by itself, and these are often a call's first)
     __device__ __forceinline__ void load_cut(const T *row, int c, int n) {
-        const int at = c < n - N ? c : n - N, s = c - at;
+        const int at = c < n - N ? c : n - N;
         u = *reinterpret_cast<const unaligned_t *>(row + at);
-        constexpr int ODD = sizeof(T) == 2 ? 1 : 0;                          // elements to a word: 2 or 1
+        shift_down(c - at);
+    }
+    // element s comes first, zeros last
+    __device__ __forceinline__ void shift_down(int s) {
+        constexpr int ODD = sizeof(T) == 2 ? 1 : 0;                          // log2 of the elements in a word
         if constexpr (ODD)
             u = s & 1 ? u32x4{__builtin_amdgcn_alignbit(u[1], u[0], 16), __builtin_amdgcn_alignbit(u[2], u[1], 16), __builtin_amdgcn_alignbit(u[3], u[2], 16), u[3] >> 16} : u;
         u = (s >> ODD) & 1 ? u32x4{u[1], u[2], u[3], 0u} : u;
