@@ -660,9 +660,10 @@ template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T 
         Chunk<T> d, v;
         d.zero();
         if (c < N) {
-            d.load(dy + m * lddy, c, N);
+            const bool wide = N >= Chunk<T>::N;
+            if (wide) d.load_cut(dy + m * lddy, c, N); else d.load(dy + m * lddy, c, N);
             if (z) {
-                v.load(z + m * ldz, c, N);
+                if (wide) v.load_cut(z + m * ldz, c, N); else v.load(z + m * ldz, c, N);
 #pragma unroll
                 for (int j = 0; j < Chunk<T>::N; ++j) {
                     const float zz = (float)v.e[j];
