@@ -62,21 +62,15 @@ template <int NV> __device__ __forceinline__ void act_apply(float (&v)[NV], int 
 // dy times GELU' = Phi(z) + z phi(z) or SILU' = s (1 + z (1 - s)), s = 1 / (1 + e^-z).  Both slopes are w(|z|) below 0 and 1 - w(|z|) above:
 // the 1 goes into the product's own rounding.  dz is rounded to 16 bits, and every value that a slope's error sends to the other
 // neighbour is a whole step in dW's sums.  (With a slope 1e-7 off, dW of 32768 x 1024 -> 4096 with GELU was 6.3e-6 off; so 0.6e-6, where
-// f32 formulas with a library's erf leave 3.7e-6.)  The pass is bound by memory and does not notice.
-__device__ __forceinline__ float act_grad(float dy, float z, int act) {
-    const float x = fabsf(z) > 128.f ? 128.f : fabsf(z); // (beyond, w is 0 to the last bit, and infinity times 0 is not)
-    float w;
-    if (act == PS_ACT_GELU) {
-        w = fmaf(x * -0.39894228f, __builtin_amdgcn_exp2f(-0.72134752f * z * z), normal_tail(z));
-    } else {
-        // e^-x as 2^t (1 + what t's rounding and log2 e's leave), 1 / (1 + e) as r + c, so that 1 - x / (1 + e) is exact at its zero
-        const float t = -1.44269504f * x, p = __builtin_amdgcn_exp2f(t);
-        const float e = fmaf(p, 0.69314718f * fmaf(-1.92596299e-8f, x, fmaf(-1.44269504f, x, -t)), p), d = 1.f + e;
-        const float r = __builtin_amdgcn_rcpf(d), c = r * fmaf(-r, e - (d - 1.f), fmaf(-d, r, 1.f));
-        w = e * (r + c) * fmaf(-x, c, fmaf(-x, r, 1.f));
-    }
-    const float dz = z < 0.f ? dy * w : fmaf(-dy, w, dy);
-    return dz == dz ? dz : dy * (z < 0.f ? w : 1.f - w);                     // (an infinite dy is one behind a slope, too)
+// f32 formulas with a library's erf leave 3.7e-6.)
+__device__ __forceinline__ float slope_below(float z, int act) {             // w; 0 to the last bit beyond 128, where infinity times 0 is not
+    if (act == PS_ACT_GELU) return fmaf(fminf(fabsf(z), 128.f) * -0.39894228f, __builtin_amdgcn_exp2f(-0.72134752f * z * z), normal_tail(z));
+    // e^-x as 2^t (1 + what t's rounding and log2 e's leave), 1 / (1 + e) as r + c, so that 1 - x / (1 + e) is exact at its zero
+    const float x = fabsf(z) > 128.f ? 128.f : fabsf(z);
+    const float t = -1.44269504f * x, p = __builtin_amdgcn_exp2f(t);
+    const float e = fmaf(p, 0.69314718f * fmaf(-1.92596299e-8f, x, fmaf(-1.44269504f, x, -t)), p), d = 1.f + e;
+    const float r = __builtin_amdgcn_rcpf(d), c = r * fmaf(-r, e - (d - 1.f), fmaf(-d, r, 1.f));
+    return e * (r + c) * fmaf(-x, c, fmaf(-x, r, 1.f));
 }
 
 // workgroup -> tile so that an XCD (workgroup id mod 8) owns a contiguous range of tiles: its L2 then serves the tiles' shared rows
@@ -660,14 +654,28 @@ template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T 
         Chunk<T> d, v;
         d.zero();
         if (c < N) {
-            const bool wide = N >= Chunk<T>::N;
-            if (wide) d.load_cut(dy + m * lddy, c, N); else d.load(dy + m * lddy, c, N);
+            if (!z && N >= Chunk<T>::N) d.load_cut(dy + m * lddy, c, N); else d.load(dy + m * lddy, c, N);
             if (z) {
-                if (wide) v.load_cut(z + m * ldz, c, N); else v.load(z + m * ldz, c, N);
+                v.load(z + m * ldz, c, N);
+                if (act == PS_ACT_RELU) {
 #pragma unroll
-                for (int j = 0; j < Chunk<T>::N; ++j) {
-                    const float zz = (float)v.e[j];
-                    d.e[j] = act == PS_ACT_RELU ? (zz > 0.f ? d.e[j] : (T)0.f) : (T)act_grad((float)d.e[j], zz, act);
+                    for (int j = 0; j < Chunk<T>::N; ++j) d.e[j] = (float)v.e[j] > 0.f ? d.e[j] : (T)0.f;
+                } else {
+                    float o[Chunk<T>::N], any = 0.f;
+#pragma unroll
+                    for (int j = 0; j < Chunk<T>::N; ++j) {
+                        const float g = (float)d.e[j], zz = (float)v.e[j], w = slope_below(zz, act);
+                        o[j] = zz < 0.f ? g * w : fmaf(-g, w, g);
+                        any += o[j];
+                    }
+                    if (any != any)                  // an infinite dy is one behind a slope, too: inf - inf w is not
+#pragma unroll
+                        for (int j = 0; j < Chunk<T>::N; ++j) {
+                            const float g = (float)d.e[j], zz = (float)v.e[j], w = slope_below(zz, act);
+                            o[j] = g * (zz < 0.f ? w : 1.f - w);
+                        }
+#pragma unroll
+                    for (int j = 0; j < Chunk<T>::N; ++j) d.e[j] = (T)o[j];
                 }
             }
         }
