@@ -338,6 +338,32 @@ def test_activations_at_their_ends(pool, t):
         assert (slope[zv == -np.inf] == 0).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("a", [R.GELU, R.SILU])
+def test_infinite_gradients_behind_a_slope(pool, t, a):
+    """an infinite dy is infinite behind a slope that is not zero, with the product's sign; its neighbours are what they were"""
+    from ps_amd import native as N
+    L, kv = N.lib(), pool.kv
+    kv.create_fc(0, 1, 1)
+    kv.put("fc0.weights", [1.0])
+    z = np.tile([-3.0, -0.5, 0.25, 1.0, 2.0, 5.0, -1e4, 1e4], 3)
+    dy = np.ones_like(z)
+    dy[8:16], dy[16] = np.inf, -np.inf
+    B = z.size
+    x, zr, d = (pool.rows(t, B, 1, values=v[:, None]) for v in (np.ones(B), z, dy))
+    dx, g = pool.rows(t, B, 1), pool.rows(R.F32, 2, 1)
+    N.check(L.ps_fc_res_backward(kv.h, 0, t, a, x.p, 1, zr.p, 1, d.p, 1, B, None, 0, dx.p, 1, g.p))
+    with np.errstate(over="ignore"):
+        got, slope = dx.get()[:, 0], R.act_grad(R.rounded(z, t), a)
+    for i in range(B):
+        if np.isfinite(dy[i]):
+            within(got[i], slope[i], 14 * R.U * (1 + min(abs(z[i]), 8)) + R.store_tol(abs(slope[i]) * 1.001, t), "row %d" % i)
+        elif abs(z[i]) < 100:
+            assert got[i] == dy[i] * np.sign(slope[i]), (i, got[i])
+        else:
+            assert got[i] == np.inf if z[i] > 0 else np.isnan(got[i])         # (infinity times 0)
+
+
 def test_pending_gradients_updaters_and_keys(pool, orc):
     """two backward calls add up in the store's pending gradients (KVStore.sum), dense_update divides by their number and runs every
     tensor's own updater; the keys are read, written, pushed and sized like the FC layers'"""
