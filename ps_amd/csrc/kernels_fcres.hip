@@ -146,8 +146,8 @@ template <> struct Weights<float> {
 // G > 1: the groups share the sum out -- for outputs of few tiles, whose chain of steps is what a call costs -- and add up through LDS, in
 // group order.
 // The product is formed transposed (weights as the first operand): a lane then holds 4 neighbouring columns of one row of y.
-// Measured: f32, 4096 x 429 -> 512, relu, z kept 22 us (82 TF; matrix units busy 0.63 of the launch, the rest is its start, first loads
-// and end; the order and number of accumulators makes no difference), 8192 x 2048 -> 2048 567 us (121 TF, 0.82 of a library's bare
+// Measured: f32, 4096 x 429 -> 512, relu, z kept 21 us (84 TF; matrix units busy 0.64 of the launch, the rest is its start, first loads
+// and end; the order and number of accumulators makes no difference), 8192 x 2048 -> 2048 550 us (125 TF, 0.85 of a library's bare
 // product); bf16, 4096 x 429 -> 512 10 us.
 template <typename T, int BM, int BN, int AHEAD, int G>
 __device__ __forceinline__ void fc_nt_tile(const FcNtArgs &a, int tiles_n, int tile, u32x4 *lds) {
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256 * G, BM == 64 ? 4 : 2) void k_fc_nt(FcNtArgs a,
 // Few rows (or few tiles): one workgroup of 16 waves per 16 columns and 16 FM rows.  The waves share out the sum in steps and take their
 // fragments straight from memory -- the weights in f32, rounded in registers, each read once per row of tiles -- so that a call is two
 // dependent trips to memory and not a chain of staged steps; their sums meet in LDS and are added in wave order.
-// Bound by latency: 3.4 us on the device for one row of 429 -> 512, 6.8 us for bf16, 16 x 2048 -> 2048 (16.8 MB of weights, 2.5 TB/s).
+// Bound by latency: 3.3 us on the device for one row of 429 -> 512, 6.6 us for bf16, 16 x 2048 -> 2048 (16.8 MB of weights, 2.5 TB/s).
 template <typename T> struct MmaFew {
     static constexpr int KS = 32;
     static __device__ __forceinline__ f32x4 mma(const Chunk<T> &a, const Chunk<T> &b, f32x4 c) {
@@ -461,7 +461,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 // Rows of x behind the last read as zeros through the buffer's bound; a last step that K does not fill goes through registers, where
 // its tail is cut off.
 // Measured: bf16, 8192 x 8192 -> 8192 1320 TF, 32768 x 4096 -> 1024 1190 (a library's bare products 1330 and 1240): the clock that the power
-// limit leaves bounds these.  32768 x 1024 -> 4096 with GELU and z kept 319 us (860 TF): 16 steps of 64 are 20 us of a tile's 38, its first
+// limit leaves bounds these.  32768 x 1024 -> 4096 with GELU and z kept 318 us (865 TF): 16 steps of 64 are 20 us of a tile's 38, its first
 // loads, GELU's arithmetic and the stores the rest, and nothing overlaps them: two workgroups a CU of 256 x 128 tiles in steps of 32 do,
 // but their loop runs at 990 TF where this one has 1320, and lose (377 us).
 template <typename T, int BN>
@@ -644,7 +644,7 @@ __global__ __launch_bounds__(512, 2) void k_fc_nt_big(FcNtArgs a, const T *Wc, i
 }
 
 // dz = dy act'(z), rounded to the type; z NULL: a copy.  dz's rows are 16-byte pieces, zeros behind the width.  Bound by memory: bf16,
-// 32768 x 4096 148 us, 5.4 TB/s.  (dz is read by both products of the pass, many times over: forming it on the way into each of them
+// 32768 x 4096 147 us, 5.5 TB/s.  (dz is read by both products of the pass, many times over: forming it on the way into each of them
 // would cost its arithmetic once per tile.)
 template <typename T> __global__ __launch_bounds__(256) void k_act_grad(const T *dy, int64_t lddy, const T *z, int64_t ldz, T *dz, int64_t lddz, int M, int N, int act) {
     const int64_t per = lddz / Chunk<T>::N, total = per * M;

@@ -10,8 +10,8 @@
 // hold up to 16 elements each: a narrow row does not idle a wave, a wide one does not spill.  Rows wider than 8192 take the kernels
 // that walk the row again (from L2).  EDGE: the width is no multiple of a 16-byte piece, so the last piece is cut off;
 // without it a lane behind the row's end reads the row's first piece and counts it as zeros, and no load hides behind a branch.
-// Measured: bf16, 65536 x 1024 forward 63 us (4.2 TB/s), backward with skip 111 us (4.9 TB/s; a copy of 1 GiB runs at 5.1); f32,
-// 4096 x 429 forward 7 us; one row 2.8 us on the device, and 7 with the call's host side.
+// Measured: bf16, 65536 x 1024 forward 51 us (5.3 TB/s; a copy of 1 GiB runs at 5.1), backward with skip 108 us (5.0 TB/s), 65536 x 1001
+// 115; f32, 4096 x 429 forward 5 us; one row 1.9 us on the device, and 7 with the call's host side.
 #include "kernels_tower.h"
 
 namespace {
