@@ -3,8 +3,8 @@
     python -m ps_amd.build [--force]
 
 One hipcc -c per translation unit (cached by mtime), then one link.  The
-library is kept in-tree (ps_amd/lib/libps_amd.so): git-ignored, but it
-travels to the GPU box with the gpurun snapshot.
+library is kept in-tree (ps_amd/lib/libps_amd.so): git-ignored, and
+goes where a copy of the tree goes.
 """
 import os
 import subprocess

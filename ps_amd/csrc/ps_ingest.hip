@@ -441,7 +441,7 @@ extern "C" int ps_libsvm_parse(const char *text, size_t len, const ps_ingest_con
 //   * a COPIER thread takes the parsed batches in order: waits until the kernels that read the slot's previous batch are done (an
 //     event the training thread recorded), ONE hipMemcpyAsync of the whole block, an event behind it -- and goes on to the next
 //     batch; a COMPLETER thread waits for those events in order and marks the batches ready.  (One thread that copied AND waited
-//     was the pipeline's limit: 167 us per batch, 24 M lines/s, with the parsers at 138 M -- first measurement of this round.)
+//     was the pipeline's limit: 167 us per batch, 24 M lines/s, with the parsers at 138 M when it was.)
 //   * ps_ingest_next hands out batch b when it is ready and gives batch b - 2's slot back to the parsers (its consumers were
 //     enqueued before this call: "valid until the call after the next one").
 // The ring holds RING batches (2 x threads, 4..64): that many batches may be in flight between the parsers and the step.
