@@ -1176,7 +1176,15 @@ template <typename T> NtKind nt_kind(const FcNtArgs &a) {
 }
 template <typename T> int nt_t(const FcNtArgs &a, hipStream_t st) {
     const NtKind k = nt_kind<T>(a);
-    if (k == NT_FEW) return a.M <= 16 ? few_go<T, 1>(a, st) : a.M <= 32 ? few_go<T, 2>(a, st) : few_go<T, 4>(a, st);
+    if (k == NT_FEW) {
+        // more rows a workgroup read the weights less often, fewer fill the chip: as many as leave 160 workgroups (us by 64 / 32 / 16 rows
+        // and how many workgroups: bf16, 64 x 2048 -> 2048 11.2 (128) / 7.6 (256); f32, 146 x 1979 -> 246 17.1 (48) / 9.8 (80) / 7.5 (160),
+        // 128 x 1024 -> 512 10.8 (64) / 6.9 (128) / 5.0 (256); f16, 2000 x 2000 -> 40 10.0 (96) / 7.3 (189) / 10.0 (375))
+        const int64_t tn = cdiv(a.N, 16);
+        if (a.M > 32 && tn * cdiv(a.M, 64) >= 160) return few_go<T, 4>(a, st);
+        if (a.M > 16 && tn * cdiv(a.M, 32) >= 160) return few_go<T, 2>(a, st);
+        return few_go<T, 1>(a, st);
+    }
     if (k == NT_128) return nt_go<T, 128, 128, sizeof(T) == 4 ? 2 : 1, 1>(a, st);
     if constexpr (sizeof(T) == 2) {
         if (k == NT_64_SPLIT) return nt_go<T, 64, 64, 2, 4>(a, st);
