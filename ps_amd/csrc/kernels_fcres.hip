@@ -1231,7 +1231,9 @@ int launch_act_grad(int type, int act, const void *dy, int64_t lddy, const void 
 // rows of 8-element multiples out and tells where).  The 256 tiles: such pieces, offsets of 31 bits inside a part, parts of at least 16
 // steps, one workgroup for each of the 256 CUs; a copy is paid for from 256 columns of the other operand on.  The smaller ones: two
 // workgroups a CU, no part shorter than four steps, and 128 only where parts stay eight steps long -- shorter ones are all start and end
-// (bf16, 4096 x 429 -> 512: 34 us in parts of 4 steps of 128, 24 by 64; 16384 x 1001 -> 1001 in parts of 32: 159 / 343).
+// (bf16, 4096 x 429 -> 512: 34 us in parts of 4 steps of 128, 24 by 64; 16384 x 1001 -> 1001 in parts of 32: 159 / 343).  16-bit parts below 12
+// steps: one workgroup a CU, whose slabs are half as many (two / one: bf16, both gradients of 4096 x 512 -> 256 19.2 / 16.5 us, of
+// 4096 x 429 -> 512 24.0 / 21.5, dW alone 16.1 / 14.4 and 19.5 / 18.5; f32, whose steps are long, 49.8 / 59.6).
 void fc_tn_plan(int type, FcTnArgs &a) {
     const bool f32 = type == PS_T_F32;
     const int64_t big = (int64_t)cdiv(a.N, 256) * cdiv(a.K, 256), steps = cdiv(a.M, 64);
@@ -1250,6 +1252,7 @@ void fc_tn_plan(int type, FcTnArgs &a) {
     for (a.tile = 128;; a.tile = 64) {
         const int64_t tiles = (int64_t)cdiv(a.N, a.tile) * cdiv(a.K, a.tile);
         int64_t s = 512 / tiles;                 // (rounded down: one workgroup too many is a round too many)
+        if (!f32 && a.tile == 64 && st < 12 * s && tiles < 256) s = 256 / tiles;
         if (s > st / 4) s = st / 4;
         a.nsplit = (int)(s < 1 ? 1 : s);
         if (a.tile == 64 || st >= 8 * a.nsplit) return;
