@@ -2,7 +2,8 @@
 
     python -m ps_amd.build [--force]
 
-One hipcc -c per translation unit (cached by mtime), then one link.  The
+One hipcc -c per translation unit (compiled again when a source, a header or
+its command line has changed), then one link.  The
 library is kept in-tree (ps_amd/lib/libps_amd.so): git-ignored, and
 goes where a copy of the tree goes.
 """
@@ -79,6 +80,20 @@ def kernel_resources():
     return out
 
 
+# What an object was compiled with, beside it: a flag like -packed-fp32-ops has to reach the units whose sources nobody touched, too.
+# (Without the paths: a tree that was moved or copied is not a changed one.)
+def _flags_of(cmd):
+    return " ".join(cmd[1:cmd.index("-c")])
+
+
+def _recorded_flags(op):
+    try:
+        with open(op + ".flags") as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def build(force=False, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -91,18 +106,21 @@ def build(force=False, verbose=False):
             continue
         op = os.path.join(OBJ, src.replace(".hip", ".o"))
         objs.append(op)
-        if force or not os.path.exists(op) or not os.path.exists(op + ".resources.json") or os.path.getmtime(op) < max(os.path.getmtime(sp), hdr_t):
-            todo.append((sp, op))
+        cmd = [hipcc] + FLAGS + ["-Rpass-analysis=kernel-resource-usage"] + os.environ.get("PS_AMD_EXTRA_FLAGS", "").split() + ["-c", sp, "-o", op]
+        if (force or not os.path.exists(op) or not os.path.exists(op + ".resources.json") or os.path.getmtime(op) < max(os.path.getmtime(sp), hdr_t)
+                or _recorded_flags(op) != _flags_of(cmd)):
+            todo.append((sp, op, cmd))
 
     def compile_one(job):
-        sp, op = job
-        cmd = [hipcc] + FLAGS + ["-Rpass-analysis=kernel-resource-usage"] + os.environ.get("PS_AMD_EXTRA_FLAGS", "").split() + ["-c", sp, "-o", op]
+        sp, op, cmd = job
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
         _record_resources(op, r.stderr)
         if r.returncode != 0:
             raise subprocess.CalledProcessError(r.returncode, cmd)
+        with open(op + ".flags", "w") as f:
+            f.write(_flags_of(cmd))
 
     if todo:        # the translation units are independent: one hipcc per core
         from concurrent.futures import ThreadPoolExecutor
