@@ -6,12 +6,17 @@
 //
 // Both are bound by memory: a row is read once, lies in registers (as it came: 16 bits stay 16 bits) while its sums are formed in two
 // passes over them -- the variance from differences to the mean, never from sum x^2 -- and is written once; the next row's loads are in
-// flight meanwhile.  All arithmetic is f32.  A row belongs to TPR lanes (4, 16 or 64 of one wave, or a workgroup of 256 or 512) that
-// hold up to 16 elements each: a narrow row does not idle a wave, a wide one does not spill.  Rows wider than 8192 take the kernels
-// that walk the row again (from L2).  EDGE: the width is no multiple of a 16-byte piece, so the last piece is cut off;
-// without it a lane behind the row's end reads the row's first piece and counts it as zeros, and no load hides behind a branch.
+// flight meanwhile.  The arithmetic is f32 but for the mean, which is the exact sum's rounded once where the values are near each other: a
+// mean one step of f32 off is far off where the spread is small (constant rows of 1e5 came out up to 1.7 beside beta).  So f32 is summed
+// in f64; 8192 values of at most 11 bits are exact in f32 (bf16, 65536 x 429: 26.3 us in f64, 23.5 so).  A row belongs to TPR lanes (4, 16
+// or 64 of one wave, or a workgroup of 256 or 512) that hold up to 16 elements each: a narrow row does not idle a wave, a wide one does
+// not spill.  Rows wider than 8192 take the kernels that walk the row again (from L2).  EDGE: the width is no multiple of a 16-byte
+// piece, so the last piece is cut off; without it a lane behind the row's end reads the row's first piece and counts it as zeros, and no
+// load hides behind a branch.
 // Measured: bf16, 65536 x 1024 forward 51 us (5.3 TB/s; a copy of 1 GiB runs at 5.1), backward with skip 108 us (5.0 TB/s), 65536 x 1001
 // 115; f32, 4096 x 429 forward 5 us; one row 1.9 us on the device, and 7 with the call's host side.
+#include <type_traits>
+
 #include "kernels_tower.h"
 
 namespace {
@@ -19,7 +24,7 @@ namespace {
 constexpr int kMaxEpl = 16;            // elements of a row per lane
 
 // N sums over the TPR lanes of a row at once; slot: alternating, so that one barrier is enough
-template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float (*lds)[16][2], int &slot) {
+template <int TPR, int N, typename V, int W> __device__ __forceinline__ void row_sums(V (&v)[N], V (*lds)[16][W], int &slot) {
 #pragma unroll
     for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1)
 #pragma unroll
@@ -38,9 +43,9 @@ template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&v)[N]
         slot ^= 1;
     }
 }
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float (*lds)[16][2], int &slot) {
-    float s[1] = {v};
-    row_sums<TPR, 1>(s, lds, slot);
+template <int TPR, typename V, int W> __device__ __forceinline__ V row_sum(V v, V (*lds)[16][W], int &slot) {
+    V s[1] = {v};
+    row_sums<TPR>(s, lds, slot);
     return s[0];
 }
 
@@ -96,13 +101,17 @@ template <typename T, int TPR, int NV, bool EDGE> __device__ __forceinline__ voi
     }
 }
 
+template <typename T> using RowSum = std::conditional_t<sizeof(T) == 4, double, float>;          // of up to 8192 values that are near each other: exact
+
 template <typename T, int TPR, int NV, bool EDGE>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_fwd(LnFwdArgs a) {
     constexpr int VEC = Chunk<T>::N, RPB = TPR > 256 ? 1 : 256 / TPR;
-    __shared__ float lds[2][16][2];
-    int slot = 0;
+    __shared__ float lds[2][16][1];
+    __shared__ RowSum<T> ldsx[2][16][1];
+    int slot = 0, slotx = 0;
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const float inv_d = 1.f / (float)a.D;
+    const double inv_d64 = 1. / a.D;
     const int64_t stride = (int64_t)gridDim.x * RPB;
     int64_t r = (int64_t)blockIdx.x * RPB + sub;
     // a lane group behind the last row repeats it and writes nothing
@@ -115,13 +124,13 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_fwd(LnFwdArgs a) {
         v = next;
         if (EDGE && r >= a.B - 1) v.settle(t, a.D);
         if (r0 + stride < a.B) next.load((const T *)a.x + (r + stride < a.B ? r + stride : a.B - 1) * a.ldx, t, a.D, r + stride >= a.B - 1);
-        float s = 0.f;
+        RowSum<T> sx = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s += inside<TPR, VEC, EDGE>(t, i, j, a.D) ? (float)v.c[i].e[j] : 0.f;
-        const float mean = row_sum<TPR>(s, lds, slot) * inv_d;
-        s = 0.f;
+            for (int j = 0; j < VEC; ++j) sx += inside<TPR, VEC, EDGE>(t, i, j, a.D) ? (float)v.c[i].e[j] : 0.f;
+        const float mean = (float)(row_sum<TPR>(sx, ldsx, slotx) * inv_d64);
+        float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -144,21 +153,25 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_fwd(LnFwdArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_ln_fwd_wide(LnFwdArgs a) {
     constexpr int VEC = Chunk<T>::N;
-    __shared__ float lds[2][16][2];
-    int slot = 0;
+    __shared__ float lds[2][16][1];
+    __shared__ double lds64[2][16][1];
+    int slot = 0, slot64 = 0;
     const float inv_d = 1.f / (float)a.D;
+    const double inv_d64 = 1. / a.D;
     for (int64_t r = blockIdx.x; r < a.B; r += gridDim.x) {
         const T *x = (const T *)a.x + r * a.ldx;
         T *y = (T *)a.y + r * a.ldy;
         Chunk<T> v;
-        float s = 0.f;
+        double s64 = 0.;
         for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.D; c += 256 * VEC) {
             v.load(x, (int)c, a.D);
+            RowSum<T> sx = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s += (float)v.e[j];
+            for (int j = 0; j < VEC; ++j) sx += (float)v.e[j];
+            s64 += sx;
         }
-        const float mean = row_sum<256>(s, lds, slot) * inv_d;
-        s = 0.f;
+        const float mean = (float)(row_sum<256>(s64, lds64, slot64) * inv_d64);
+        float s = 0.f;
         for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.D; c += 256 * VEC) {
             v.load(x, (int)c, a.D);
 #pragma unroll
@@ -229,7 +242,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_ln_bwd(LnBwdArgs a) {
                 sg[i * VEC + j] = fmaf(d, h, sg[i * VEC + j]); sb[i * VEC + j] += d;
             }
         if (!a.dx) continue;
-        row_sums<TPR, 2>(s, lds, slot);
+        row_sums<TPR>(s, lds, slot);
         if (!live) continue;
         const float m1 = s[0] * inv_d, m2 = s[1] * inv_d;
 #pragma unroll

@@ -1,0 +1,69 @@
+"""How near the residual tower's operators come to their definitions where f32 formulas usually lose: the activations' tails, rows far
+from zero with little or no variance.  The bounds are derived here, beside each test."""
+import numpy as np
+import pytest
+
+import tower_ref as R
+from test_gpu_tower import EPS, Pool, within
+
+pytestmark = pytest.mark.gpu
+f32, U = np.float32, R.U
+TYPES = [R.F32, R.BF16, R.F16]
+
+
+@pytest.fixture
+def pool():
+    p = Pool()
+    yield p
+    p.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("D", [3, 7, 24, 49, 107, 300, 429, 512, 1001, 1024, 2051, 4099, 8191, 9001])
+def test_ln_of_constant_rows_is_beta(pool, t, D):
+    """a row of one value has no variance: whatever the value, y is beta (the mean of equal f32 numbers is that number, and x - mean is 0
+    exactly), and 1 / sqrt(var + eps) that of eps.  A mean that is a step off is divided by sqrt(eps) = 0.003 and shows."""
+    from ps_amd import native as N
+    L, kv = N.lib(), pool.kv
+    rng = np.random.default_rng(D)
+    c = np.array([1.0, -3.5, 0.1, 1000.0, 1e5 if t != R.F16 else 6e4, -12345.678, 3e-3, 77.7])
+    B = c.size
+    v = np.tile(c[:, None], (1, D))
+    g, b = (1 + 0.2 * rng.standard_normal(D)).astype(f32), (0.2 * rng.standard_normal(D)).astype(f32)
+    kv.create_ln(0, D)
+    kv.put("ln0.weights", g)
+    kv.put("ln0.bias", b)
+    xr, yr, st = pool.rows(t, B, D, values=v), pool.rows(t, B, D), pool.rows(R.F32, B, 2)
+    N.check(L.ps_ln_forward(kv.h, 0, t, xr.p, D, B, EPS, yr.p, D, st.p))
+    np.testing.assert_array_equal(yr.get(), np.tile(R.rounded(b, t), (B, 1)))
+    s = st.get()
+    np.testing.assert_array_equal(s[:, 0], R.rounded(c, t))
+    within(s[:, 1], np.full(B, 1 / np.sqrt(np.float64(f32(EPS)))), 3 * U / np.sqrt(EPS), "rstd")
+
+
+@pytest.mark.parametrize("t", [R.F32, R.BF16])
+@pytest.mark.parametrize("D", [24, 300, 1024, 2051, 9001])
+def test_ln_far_from_zero(pool, t, D):
+    """rows whose mean is far larger than their spread: what is lost is the rounding of the mean to f32 (u |mean|), not a whole sum's.
+    d = x - m is exact up to u |d| for any m near the values, m' = m + mean(d) is off by u |mean| and the chain of d's sum, (c + 2) u
+    mean|d| -- c the longest chain of adds, ln_chain -- and y carries that over the spread."""
+    from ps_amd import native as N
+    L, kv = N.lib(), pool.kv
+    rng = np.random.default_rng(D + 1)
+    B = 5
+    x = rng.standard_normal((B, D)) * (1.0 if t == R.F32 else 400.0) + np.array([1e4, -3e4, 1e5, 7e3, 12.0])[:, None]
+    kv.create_ln(0, D)
+    xr, yr, st = pool.rows(t, B, D, values=x), pool.rows(t, B, D), pool.rows(R.F32, B, 2)
+    N.check(L.ps_ln_forward(kv.h, 0, t, xr.p, D, B, EPS, yr.p, D, st.p))
+    x = R.rounded(x, t)
+    y, mean, rstd = R.ln_forward(x, 1.0, 0.0, f32(EPS))
+    c = R.ln_chain(D)
+    spread = np.abs(x - mean).mean(1, keepdims=True)
+    # the first mean m is off by at most (c + 2) u mean|x|, which d's sum then carries in every term
+    d = spread + (c + 2) * U * np.abs(x).mean(1, keepdims=True)
+    e = U * np.abs(mean) + (c + 4) * U * d
+    rel = 0.5 * (2 * d * d * (c + 8) * U * rstd ** 2 + (c + 4) * U) + 6 * U
+    tol = e * rstd + np.abs(y) * (rel + 4 * U)
+    s = st.get()
+    within(s[:, :1], mean, e, "mean")
+    within(yr.get(), y, tol + R.store_tol(np.abs(y) + tol, t), "y")
