@@ -67,3 +67,29 @@ def test_ln_far_from_zero(pool, t, D):
     s = st.get()
     within(s[:, :1], mean, e, "mean")
     within(yr.get(), y, tol + R.store_tol(np.abs(y) + tol, t), "y")
+
+
+def through_one(pool, t, a, z):
+    """(z as the type has it, act(z), act'(z)) by a product with the number 1"""
+    from ps_amd import native as N
+    L, kv = N.lib(), pool.kv
+    kv.create_fc(0, 1, 1)
+    kv.put("fc0.weights", [1.0])
+    kv.put("fc0.bias", [0.0])
+    B = z.size
+    zr, y, dy = pool.rows(t, B, 1, values=z[:, None]), pool.rows(t, B, 1), pool.rows(t, B, 1, values=np.ones((B, 1)))
+    dx, g = pool.rows(t, B, 1), pool.rows(R.F32, 2, 1)
+    N.check(L.ps_fc_res_forward(kv.h, 0, t, a, zr.p, 1, B, None, 0, None, 0, y.p, 1))
+    N.check(L.ps_fc_res_backward(kv.h, 0, t, a, zr.p, 1, zr.p, 1, dy.p, 1, B, None, 0, dx.p, 1, g.p))
+    return R.rounded(z, t), y.get()[:, 0], dx.get()[:, 0]
+
+
+def test_silu_f32_is_accurate_relative_to_itself(pool):
+    """z / (1 + e^-z) in f32, from e = e^-|z|: e is off by 3 u (the exponential a step, its correction half of one), 1 + e by u and its
+    reciprocal by u, and a value below 0 has two products more: 7 u of the value.  Beyond -87.3 e is below f32's normal numbers and the
+    value, less than 1.1e-36, becomes 0.  (e^0 is exact, the value at 0 too.)"""
+    z = np.concatenate([-np.logspace(-6, np.log10(120), 3000), np.logspace(-6, 2, 1000), np.random.default_rng(0).standard_normal(4000) * 3])
+    zv, y, _ = through_one(pool, R.F32, R.SILU, z)
+    e = np.exp(-np.abs(zv))
+    want = zv * np.where(zv < 0, e, 1.0) / (1 + e)
+    within(y, want, 7.01 * U * np.abs(want) + 1.1e-36, "silu")
