@@ -59,6 +59,8 @@ __device__ __forceinline__ float silu_f32(float z) {
     const float x = fminf(fabsf(z), 128.f), e = exp_minus(x), d = 1.f + e, r = __builtin_amdgcn_rcpf(d);
     return (z < 0.f ? -x * e : z) * fmaf(r, fmaf(-d, r, 1.f), r);
 }
+// a product in which 0 times infinity is 0 (a NaN stays one): one instruction, like any product
+extern "C" __device__ float mul_zero_wins(float, float) __asm("llvm.amdgcn.fmul.legacy");
 template <typename T, int NV> __device__ __forceinline__ void act_apply(float (&v)[NV], int act) {
     if (act == PS_ACT_RELU) {
 #pragma unroll
@@ -71,7 +73,7 @@ template <typename T, int NV> __device__ __forceinline__ void act_apply(float (&
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if constexpr (sizeof(T) == 4) v[j] = silu_f32(v[j]);
-            else v[j] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v[j]));
+            else v[j] = mul_zero_wins(v[j], __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v[j])));      // (0 at -infinity)
     }
 }
 // dy times GELU' = Phi(z) + z phi(z) or SILU' = s (1 + z (1 - s)), s = 1 / (1 + e^-z).  Both slopes are w(|z|) below 0 and 1 - w(|z|) above:

@@ -93,3 +93,10 @@ def test_silu_f32_is_accurate_relative_to_itself(pool):
     e = np.exp(-np.abs(zv))
     want = zv * np.where(zv < 0, e, 1.0) / (1 + e)
     within(y, want, 7.01 * U * np.abs(want) + 1.1e-36, "silu")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("a", [R.GELU, R.SILU])
+def test_activations_at_minus_infinity_are_their_limits(pool, t, a):
+    _, y, slope = through_one(pool, t, a, np.array([-np.inf, -1e30, -3e4, np.nan, 1.0]))
+    assert (y[:3] == 0).all() and (slope[:3] == 0).all() and np.isnan(y[3]) and abs(y[4]) > 0.5
