@@ -32,18 +32,21 @@ template <> struct Mma<float> {        // a fragment holds 4 steps of 2: the lan
 };
 
 // The normal law's tail Q(|z|) = erfc(|z| / sqrt 2) / 2 as 2 to a polynomial of |z|: log2 Q is nearly a parabola, and the polynomial is the
-// one of degree 8 whose greatest |error of Q| on [0, 6] is least; it falls from there on.  |error| < 4e-8, the rounding of numbers
-// near 1/2 (relative below 2e-6 up to 3, 2e-4 at 4), from 8 multiply-adds and one exponential: in the epilogue of a product nothing
-// hides them.
+// one of degree 10 whose error on [0, 8] is least, weighed as Q's own error or, where that is more, a twentieth of Q's in percent; it
+// falls from there on.  In f32: |error| < 5e-8, the rounding of numbers near 1/2, and below 4e-4 of Q up to 8 (1e-6 up to 2, 6e-6 up to 3,
+// 4e-5 up to 4): a 16-bit GELU is its value rounded once down to -8, where it is 5e-15, and an ever smaller number below.  10
+// multiply-adds and one exponential: in the epilogue of a product nothing hides them.
 __device__ __forceinline__ float normal_tail(float z) {
     const float x = fabsf(z);
-    float p = fmaf(-2.77219374e-6f, x, 3.86222273e-5f);
-    p = fmaf(p, x, -1.82553558e-4f);
-    p = fmaf(p, x, -1.45858037e-4f);
-    p = fmaf(p, x, 7.07545876e-3f);
-    p = fmaf(p, x, -0.0525050201f);
-    p = fmaf(p, x, -0.459204912f);
-    p = fmaf(p, x, -1.15110576f);
+    float p = fmaf(-1.76279684e-08f, x, 6.04504919e-07f);
+    p = fmaf(p, x, -8.63394234e-06f);
+    p = fmaf(p, x, 6.51972878e-05f);
+    p = fmaf(p, x, -0.00024829671f);
+    p = fmaf(p, x, -5.21555776e-05f);
+    p = fmaf(p, x, 0.00699824048f);
+    p = fmaf(p, x, -0.0524695776f);
+    p = fmaf(p, x, -0.459213197f);
+    p = fmaf(p, x, -1.15110493f);
     return __builtin_amdgcn_exp2f(fmaf(p, x, -1.f));
 }
 // e^-x for 0 <= x <= 128 as 2^t (1 + what t's rounding and log2 e's leave)
@@ -67,8 +70,8 @@ template <typename T, int NV> __device__ __forceinline__ void act_apply(float (&
         for (int j = 0; j < NV; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];        // (a NaN stays one)
     } else if (act == PS_ACT_GELU) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)             // z Phi(z) = max(z, 0) - |z| Q(|z|), and Q(64) is 0 (so is Q(infinity) times it)
-            v[j] = fmaf(-fminf(fabsf(v[j]), 64.f), normal_tail(v[j]), fmaxf(v[j], 0.f));
+        for (int j = 0; j < NV; ++j)             // z Phi(z) = max(z, 0) - |z| Q(|z|), the first as whole numbers (fmaxf is two instructions)
+            v[j] = __int_as_float(max(__float_as_int(v[j]), 0)) - mul_zero_wins(fabsf(v[j]), normal_tail(v[j]));
     } else if (act == PS_ACT_SILU) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)

@@ -2,6 +2,7 @@
 from zero with little or no variance.  The bounds are derived here, beside each test."""
 import numpy as np
 import pytest
+from scipy.special import erfc
 
 import tower_ref as R
 from test_gpu_tower import EPS, Pool, within
@@ -100,3 +101,21 @@ def test_silu_f32_is_accurate_relative_to_itself(pool):
 def test_activations_at_minus_infinity_are_their_limits(pool, t, a):
     _, y, slope = through_one(pool, t, a, np.array([-np.inf, -1e30, -3e4, np.nan, 1.0]))
     assert (y[:3] == 0).all() and (slope[:3] == 0).all() and np.isnan(y[3]) and abs(y[4]) > 0.5
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_gelu_tail_is_rounded_once(pool, t):
+    """z Phi(z) for z < 0 is -|z| Q(|z|).  Q's polynomial in f32 arithmetic (test_tower_accuracy_cpu.py evaluates it) is within 5e-8 of Q
+    and, down to -8, within 4e-4 of it relatively; the exponential adds a step (2 u) and the product half of one.  In 16 bits that is the
+    storing's rounding and a fifth of it, down to -8, where the value is 5e-15; from there on it is smaller than that."""
+    z = -np.concatenate([np.linspace(0.01, 14, 3000), np.random.default_rng(1).random(1000) * 8])
+    zv, y, slope = through_one(pool, t, R.GELU, z)
+    q = 0.5 * erfc(-zv / np.sqrt(2.0))
+    off = np.where(zv >= -8, np.minimum(5e-8, 4e-4 * q), q)
+    tol = np.abs(zv) * off + 4 * U * np.abs(zv) * q
+    within(y, zv * q, tol + R.store_tol(np.abs(zv * q) + tol, t), "gelu")
+    # the slope Q - |z| phi: Q as above; |z| phi by an exponential of z^2 log2(e) / 2, whose argument carries 2 u of itself
+    p = np.abs(zv) * np.exp(-zv * zv / 2) / np.sqrt(2 * np.pi)
+    want = q - p
+    tol = off + 4 * U * q + (zv * zv + 6) * U * p + 2e-37
+    within(slope, want, tol + R.store_tol(np.abs(want) + tol, t), "slope")
