@@ -19,7 +19,8 @@ def tail(x):
     x = x.astype(f32).astype(np.float64)
     p = np.full_like(x, f32(float(lead)))
     for c in [second] + rest + [last]:
-        p = (p * x + float(f32(float(c)))).astype(f32).astype(np.float64)
+        with np.errstate(over="ignore"):          # (far beyond 8: to minus infinity)
+            p = (p * x + float(f32(float(c)))).astype(f32).astype(np.float64)
     return np.exp2(p).astype(f32).astype(np.float64), len(rest) + 2
 
 
