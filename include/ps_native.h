@@ -499,6 +499,11 @@ int ps_auc_compute(ps_store_t *s, const float *p, const float *y, int64_t n, int
 /* Adopt the host framework's HIP stream (hipStream_t) for everything this
  * store enqueues, so kernels and the host's collectives are stream-ordered. */
 int ps_store_set_stream(ps_store_t *s, void *hip_stream);
+/* For a host framework that stays on a stream of its own (NULL: HIP's default stream): what the store enqueues from now on
+ * runs behind what is enqueued on hip_stream (store_first = 0), or the other way round (1).  Events, no host wait; nothing
+ * to do where it is the store's stream, or where a graph is being recorded on that.  A graph being recorded on hip_stream:
+ * PS_E_STATE (adopt the stream: what the store has enqueued lies outside the graph). */
+int ps_store_order(ps_store_t *s, void *hip_stream, int store_first);
 /* Worker: stage the batch, find its unique (field,id) keys grouped by owner
  * shard.  counts_out[nshards] = keys per owner; *send_rows_dev = the
  * owner-local row of every unique key (uint32, owner-major, ascending row).

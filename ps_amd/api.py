@@ -14,6 +14,7 @@ Arrays use the reference's byte layout: a FloatMatrix "features x B"
 compute path; nothing here falls back to numpy.
 """
 import ctypes as C
+import sys
 
 import numpy as np
 
@@ -117,6 +118,8 @@ class KVStore:
         if hasattr(obj, "_hcell"):
             self._model_cells = getattr(self, "_model_cells", []) + [obj._hcell]
 
+    stream = None              # the adopted stream's handle; None: the store's own
+
     @classmethod
     def ins(cls, device=0, seed=0):
         if device not in cls._ins:
@@ -163,6 +166,7 @@ class KVStore:
     def set_stream(self, stream):
         """Adopt a HIP stream (its handle, e.g. torch.cuda.current_stream().cuda_stream) for everything this store enqueues."""
         N.check(N.lib().ps_store_set_stream(self.h, stream))
+        self.stream = getattr(stream, "value", stream) or 0        # (None: HIP's default stream)
 
     def dense_update(self, layer=-1):
         """KVStore.update(Map) + clear for the pending gradients of the dense tensors (layer < 0: every FC layer and normalisation)."""
@@ -523,9 +527,37 @@ def _f32(t, name, shape, like):
     return t.data_ptr()
 
 
+_STREAM_OF = {}      # a tensor's class -> device number -> the handle of the stream its framework works on (None: not known)
+
+
+def _stream_of(cls):
+    torch, f = sys.modules.get("torch"), lambda device: None
+    if torch is not None and issubclass(cls, torch.Tensor):
+        f = (getattr(torch._C, "_cuda_getCurrentRawStream", None)              # 0.1 us; a Stream object is 1.5
+             or (lambda device: torch.cuda.current_stream(device).cuda_stream))
+    _STREAM_OF[cls] = f
+    return f
+
+
 class _TowerLayer:
+    """Tensors are torch's, on the store's device.  A call runs on the store's stream: torch's current one where the store has
+    adopted it (KVStore.set_stream; the only form that a graph can record).  Otherwise it is ordered behind what torch has enqueued
+    and before what torch enqueues next, allocations included, by two events."""
+
     def __init__(self, store, layer):
         self.store, self.layer = store, layer
+
+    def _call(self, x, fn, *args):
+        kv, cls = self.store, type(x)
+        cur = (_STREAM_OF.get(cls) or _stream_of(cls))(kv.device)
+        if cur is None or cur == kv.stream:
+            N.check(fn(kv.h, self.layer, *args))
+            return
+        N.check(N.lib().ps_store_order(kv.h, cur, 0))
+        try:
+            N.check(fn(kv.h, self.layer, *args))
+        finally:
+            N.check(N.lib().ps_store_order(kv.h, cur, 1))
 
     def _type(self, x):
         t = _TYPES.get(x.dtype)
@@ -550,7 +582,7 @@ class _TowerLayer:
 
 class LnLayer(_TowerLayer):
     """Layer normalisation over the rows of a [B][dims] device tensor, "ln<layer>.*" of the store.  Tensors are torch's (float32,
-    bfloat16 or float16; rows may be strided), on the store's device and ready on the store's stream (KVStore.set_stream)."""
+    bfloat16 or float16; rows may be strided), on the store's device and any stream (_TowerLayer)."""
 
     def __init__(self, store, layer, dims, eps=1e-5):
         super().__init__(store, layer)
@@ -566,7 +598,7 @@ class LnLayer(_TowerLayer):
             y = x.new_empty((B, self.dims))
         yp, ldy = _mat(y, "y", B, self.dims, x)
         sp = None if stats is None else _f32(stats, "stats", (B, 2), x)
-        N.check(N.lib().ps_ln_forward(self.store.h, self.layer, ty, xp, ldx, B, self.eps, yp, ldy, sp))
+        self._call(x, N.lib().ps_ln_forward, ty, xp, ldx, B, self.eps, yp, ldy, sp)
         return y
 
     def backward(self, x, stats, dy, skip=None, dx=None, grad=None, want_dx=True):
@@ -581,7 +613,7 @@ class LnLayer(_TowerLayer):
             dx = x.new_empty((B, self.dims))
         dxp, lddx = (None, 0) if dx is None else _mat(dx, "dx", B, self.dims, x)
         gp = None if grad is None else _f32(grad, "grad", (2, self.dims), x)
-        N.check(N.lib().ps_ln_backward(self.store.h, self.layer, ty, xp, ldx, _f32(stats, "stats", (B, 2), x), dyp, lddy, B, kp, ldk, dxp, lddx, gp))
+        self._call(x, N.lib().ps_ln_backward, ty, xp, ldx, _f32(stats, "stats", (B, 2), x), dyp, lddy, B, kp, ldk, dxp, lddx, gp)
         return dx
 
     def pending_grad(self, bias=False):
@@ -594,7 +626,7 @@ class LnLayer(_TowerLayer):
 
 class FcResLayer(_TowerLayer):
     """y = act(x W + b) + res over [B][in_dims] device tensors, "fc<layer>.*" of the store (the parameters FcLayer trains: float32;
-    16-bit activations multiply weights rounded to their type).  act: PS_ACT_NONE / RELU / GELU / SILU."""
+    16-bit activations multiply weights rounded to their type).  act: PS_ACT_NONE / RELU / GELU / SILU.  Tensors as LnLayer's."""
 
     def __init__(self, store, layer, in_dims, out_dims, act=N.PS_ACT_NONE):
         super().__init__(store, layer)
@@ -611,7 +643,7 @@ class FcResLayer(_TowerLayer):
         rp, ldr = (None, 0) if res is None else _mat(res, "res", B, self.out_dims, x)
         zp, ldz = (None, 0) if z is None else _mat(z, "z", B, self.out_dims, x)
         yp, ldy = _mat(y, "y", B, self.out_dims, x)
-        N.check(N.lib().ps_fc_res_forward(self.store.h, self.layer, ty, self.act, xp, ldx, B, rp, ldr, zp, ldz, yp, ldy))
+        self._call(x, N.lib().ps_fc_res_forward, ty, self.act, xp, ldx, B, rp, ldr, zp, ldz, yp, ldy)
         return y
 
     def backward(self, x, z, dy, skip=None, dx=None, grad=None, want_dx=True):
@@ -627,7 +659,7 @@ class FcResLayer(_TowerLayer):
             dx = x.new_empty((B, self.in_dims))
         dxp, lddx = (None, 0) if dx is None else _mat(dx, "dx", B, self.in_dims, x)
         gp = None if grad is None else _f32(grad, "grad", (self.in_dims + 1, self.out_dims), x)
-        N.check(N.lib().ps_fc_res_backward(self.store.h, self.layer, ty, self.act, xp, ldx, zp, ldz, dyp, lddy, B, kp, ldk, dxp, lddx, gp))
+        self._call(x, N.lib().ps_fc_res_backward, ty, self.act, xp, ldx, zp, ldz, dyp, lddy, B, kp, ldk, dxp, lddx, gp)
         return dx
 
     def pending_grad(self, bias=False):

@@ -470,6 +470,19 @@ extern "C" int ps_store_set_stream(ps_store_t *s, void *hip_stream) {
     return PS_OK;
 }
 
+extern "C" int ps_store_order(ps_store_t *s, void *hip_stream, int store_first) {
+    if (!s) return ps_set_err(PS_E_BAD_ARG, "store is NULL");
+    const hipStream_t other = (hipStream_t)hip_stream;
+    if (other == s->stream || (s->stream && stream_is_capturing(s->stream))) return PS_OK;
+    if (other && stream_is_capturing(other))
+        return ps_set_err(PS_E_STATE, "a graph is being recorded on a stream that is not the store's: adopt it (ps_store_set_stream) first");
+    PSCHK(store_enter(s));
+    if (!s->order_ev) HIPCHK(hipEventCreateWithFlags(&s->order_ev, hipEventDisableTiming));
+    HIPCHK(hipEventRecord(s->order_ev, store_first ? s->stream : other));
+    HIPCHK(hipStreamWaitEvent(store_first ? other : s->stream, s->order_ev, 0));
+    return PS_OK;
+}
+
 // the plan's kernels; readback: also copy owner_start to pinned memory and record plan_ev (ps_shard_plan_finish)
 // The slot of every entry (the forward reads it ~50 us later) and the entry lists of the backward (stable sort + runs),
 // on side stream 0 beside the exchange and the forward.  k_plan_slots before the sort in stream order: the general

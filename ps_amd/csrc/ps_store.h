@@ -53,6 +53,7 @@ struct ps_store {
     uint64_t seed = 0;
     hipStream_t stream = nullptr;      // the stream everything is enqueued on (own_stream, or one adopted from the host)
     hipStream_t own_stream = nullptr;
+    hipEvent_t order_ev = nullptr;     // ps_store_order
     hipStream_t prefetch_stream = nullptr;   // ps_shard_step_begin(use_side): the next step's key lists, beside training
     EmbTables emb;
     WideTable wide;

@@ -307,6 +307,7 @@ extern "C" int ps_store_destroy(ps_store_t *s) {
     sort_ws_free(s->push_ws);
     fr(s->push_keys); fr(s->push_ents); fr(s->push_seg_start); fr(s->push_seg_id); fr(s->push_nseg);
     fr(s->push_mask); fr(s->push_pos);
+    if (s->order_ev) (void)hipEventDestroy(s->order_ev);
     pool_stream_release(s->device, 1, s->own_stream);    // (an adopted stream belongs to the host: only the store's own goes back)
     pool_stream_release(s->device, 1, s->prefetch_stream);
     delete s;

@@ -133,6 +133,7 @@ SIGNATURES = {
     "ps_emb_backward_update": (_i, [_vp, _vp, _vp, _i64, _i, _i, _vp, _i, _vp, _i, _i, _i, _i]),
     "ps_emb_last_grads": (_i, [_vp, _pi64, _pf, _i64, _pi64]),
     "ps_store_set_stream": (_i, [_vp, _vp]),
+    "ps_store_order": (_i, [_vp, _vp, _i]),
     "ps_shard_plan": (_i, [_vp, C.POINTER(ps_batch_t), _i, _vp, _pi64, _pvp, _pi64]),
     "ps_shard_plan_launch": (_i, [_vp, C.POINTER(ps_batch_t), _i, _vp]),
     "ps_shard_plan_finish": (_i, [_vp, _pi64, _pvp, _pi64]),

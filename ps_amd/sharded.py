@@ -721,7 +721,7 @@ def _run_bench(args, cfg, synth_batch, stage, wd):
         gms = [ps_amd.WideDeepNN.buildModel(cfg["F"], cfg["D"], cfg["X"], cfg["fc"], cfg["wide"], store=kv, max_batch=cfg["B"])
                for _ in range(4 if overlap else 1)]       # plan contexts: steps t+1, t+2 are planned while step t trains and t-1 drains
         torch.cuda.set_stream(torch.cuda.Stream(dev))      # not the legacy null stream (implicit syncs with blocking streams)
-        N.check(L.ps_store_set_stream(kv.h, torch.cuda.current_stream().cuda_stream))
+        kv.set_stream(torch.cuda.current_stream().cuda_stream)
         comm = TorchComm(dist, torch, dev, overlap=overlap)
         threaded = overlap and bool(getattr(args, "prefetch_thread", 0))
         worker = ShardedWorker(HipBackend(gms, torch, dev), comm, is_async=bool(getattr(args, "is_async", 0)))
