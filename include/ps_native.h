@@ -173,7 +173,7 @@ enum { PS_GRAD_COMPAT = 0,     /* reference arithmetic incl. the double-backward
                                   "every wide key ever seen" gradient (A.10)   */
        PS_GRAD_INTENDED = 1    /* mean over occurrences / per-key presence sum */ };
 enum { PS_ACT_NONE = 0, PS_ACT_RELU = 1, PS_ACT_SIGMOID = 2,
-       PS_ACT_GELU = 3, PS_ACT_SILU = 4   /* the residual tower's operators only (ps_fc_res_*): z Phi(z) and z / (1 + e^-z) */ };
+       PS_ACT_GELU = 3, PS_ACT_SILU = 4   /* the residual tower's operators only (ps_fc_res_*; PS_E_UNSUPPORTED elsewhere): z Phi(z) and z / (1 + e^-z) */ };
 
 typedef struct ps_model_config {
     int kind;            /* PS_MODEL_*                                        */

@@ -94,6 +94,7 @@ extern "C" int ps_fc_backward(ps_store_t *s, int layer, int act, const float *x_
     if (ldd != p.ldw) return ps_set_err(PS_E_BAD_ARG, "fc%d wants ldd = %d (out rounded up to 16, padding columns zero)", layer, p.ldw);
     if (act != PS_ACT_NONE && (!y_dev || ldy < p.N)) return ps_set_err(PS_E_BAD_ARG, "act' needs the layer's output y_dev");
     if (dx_dev && (lddx < p.K || (lddx & 3))) return ps_set_err(PS_E_BAD_ARG, "bad lddx %d", lddx);
+    PSCHK(store_check_act(act));
     PSCHK(store_enter(s));
     hipStream_t st = s->stream;
     // activation.backward in place (:100-102)
@@ -200,6 +201,7 @@ extern "C" int ps_emb_backward_update(ps_store_t *s, const int64_t *ids_dev, con
     if (apply && !e.state && stateful)
         return ps_set_err(PS_E_STATE, "the embedding table was created weights-only (state_slots = 0): Adam / Ftrl cannot train it");
     if (nnz == 0) return PS_OK;
+    PSCHK(store_check_act(act));
     PSCHK(store_enter(s));
     hipStream_t st = s->stream;
     ps_store::OpScratch &o = s->ops;

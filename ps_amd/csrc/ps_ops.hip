@@ -50,6 +50,7 @@ extern "C" int ps_emb_forward(ps_store_t *s, const int64_t *ids_dev, const int64
     if (!s || !ids_dev || !out_dev || B <= 0) return ps_set_err(PS_E_BAD_ARG, "bad argument");
     if (!s->emb.W) return ps_set_err(PS_MISSING, "no embedding tables");
     if (ld < s->emb.F * s->emb.D || (s->emb.D % 4 == 0 && (ld & 3))) return ps_set_err(PS_E_BAD_ARG, "bad ld %d", ld);
+    PSCHK(store_check_act(act));
     PSCHK(store_enter(s));
     EmbFwdArgs e;
     memset(&e, 0, sizeof e);
@@ -68,6 +69,7 @@ extern "C" int ps_fc_forward(ps_store_t *s, int layer, int act, const float *x_d
     FcParams &p = s->fc[layer];
     if (ldx != p.Kpad) return ps_set_err(PS_E_BAD_ARG, "fc%d wants ldx = %d (in+1 rounded up to 16, ones column at %d)", layer, p.Kpad, p.K);
     if (ldy < p.N) return ps_set_err(PS_E_BAD_ARG, "ldy %d < out %d", ldy, p.N);
+    PSCHK(store_check_act(act));
     PSCHK(store_enter(s));
     const int epi = act == PS_ACT_RELU ? EPI_RELU : act == PS_ACT_SIGMOID ? EPI_SIGMOID : EPI_NONE;
     return gemm_nt(x_dev, ldx, B, p.Wt, p.Kpad, p.N, y_dev, ldy, B, p.N, p.Kpad, epi, nullptr, 0, 0, nullptr, s->stream);

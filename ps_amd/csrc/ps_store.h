@@ -106,6 +106,11 @@ static inline bool key_is_ln(const ParsedKey &k) { return k.kind >= 5; }
 // KVStore.update of a dense tensor's pending gradient (ps_layer_ops.hip); false: it has none
 int store_apply_pending(ps_store *s, FcParams &p, const char *stem, int layer, bool *done);
 #define PS_LN_MAX 64
+// the operators that know the reference's activations alone: the residual tower's would pass for none
+static inline int store_check_act(int act) {
+    if (act == PS_ACT_GELU || act == PS_ACT_SILU) return ps_set_err(PS_E_UNSUPPORTED, "GELU and SiLU are the residual tower's activations (ps_fc_res_forward)");
+    return PS_OK;
+}
 // PServer.push (+ psUpdate) of a list of (owner-local row, gradient) pairs; bump_step: globalStep.incrementAndGet()
 int shard_apply_push(ps_store *s, const uint32_t *rows_dev, const float *grads_dev, int64_t n, const int64_t *peer_counts,
                      int npeers, int is_async, bool bump_step);
