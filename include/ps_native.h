@@ -347,7 +347,11 @@ int ps_dense_update(ps_store_t *s, int layer);
  * be waiting to be joined (ps_store_sync first) -- and with grad_dev given: the
  * pending gradient's count lives on the host, so a call that would add to it is
  * refused while recording, PS_E_UNSUPPORTED.  The workspace is the store's: replays
- * of its graphs are calls on the store, one at a time like all of them. */
+ * of its graphs are calls on the store, one at a time like all of them.
+ * Limits: 8 FC tensors a store (ps_store_create_fc; a model's own among them) and 64
+ * normalisations.  A gradient in grad_dev is the caller's to apply, by way of the host
+ * (ps_store_push_update takes host memory); pending gradients are this process's own,
+ * the multi-rank step reduces a model's tensors alone. */
 enum { PS_T_F32 = 0, PS_T_BF16 = 1, PS_T_F16 = 2 };
 /* "ln<layer>.weights" = 1 / "ln<layer>.bias" = 0, dims each; layer < 64, dims <= 2^20.
  * Again with the same dims: nothing happens. */
