@@ -477,7 +477,10 @@ extern "C" int ps_store_order(ps_store_t *s, void *hip_stream, int store_first) 
     if (other && stream_is_capturing(other))
         return ps_set_err(PS_E_STATE, "a graph is being recorded on a stream that is not the store's: adopt it (ps_store_set_stream) first");
     PSCHK(store_enter(s));
-    if (!s->order_ev) HIPCHK(hipEventCreateWithFlags(&s->order_ev, hipEventDisableTiming));
+    if (!s->order_ev) {
+        RtGuard rt_guard;
+        HIPCHK(hipEventCreateWithFlags(&s->order_ev, hipEventDisableTiming));
+    }
     HIPCHK(hipEventRecord(s->order_ev, store_first ? s->stream : other));
     HIPCHK(hipStreamWaitEvent(store_first ? other : s->stream, s->order_ev, 0));
     return PS_OK;
