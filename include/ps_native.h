@@ -346,7 +346,8 @@ int ps_dense_update(ps_store_t *s, int layer);
  * does not grow while recording, PS_E_STATE, nor may a fused training step still
  * be waiting to be joined (ps_store_sync first) -- and with grad_dev given: the
  * pending gradient's count lives on the host, so a call that would add to it is
- * refused while recording, PS_E_UNSUPPORTED.  The workspace is the store's: replays
+ * refused while recording, PS_E_UNSUPPORTED, and so is a normalisation's update
+ * (ps_ln_update, ps_dense_update(s, -1)) from one.  The workspace is the store's: replays
  * of its graphs are calls on the store, one at a time like all of them.
  * Limits: 8 FC tensors a store (ps_store_create_fc; a model's own among them) and 64
  * normalisations.  A gradient in grad_dev is the caller's to apply, by way of the host

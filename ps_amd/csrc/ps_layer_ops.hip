@@ -132,6 +132,12 @@ extern "C" int ps_fc_pending_grad(ps_store_t *s, int layer, int bias, float *out
     return PS_OK;
 }
 
+// No call that adds to a normalisation's pending gradient can be recorded, so a recorded update would apply what lies there again and again
+int store_check_ln_update(ps_store *s) {
+    if (!stream_is_capturing(s->stream)) return PS_OK;
+    return ps_set_err(PS_E_UNSUPPORTED, "a normalisation's pending gradient and its count are of the moment: its update is not recorded");
+}
+
 // KVStore.update(Map): g = sum / sumCnt, updater by key (exact, prefix, "default"), then clear (:240-277)
 int store_apply_pending(ps_store *s, FcParams &p, const char *stem, int layer, bool *done) {
     *done = false;
@@ -165,6 +171,8 @@ int store_apply_pending(ps_store *s, FcParams &p, const char *stem, int layer, b
 extern "C" int ps_dense_update(ps_store_t *s, int layer) {
     RoctxRange roctx_range("ps_dense_update");
     if (!s) return ps_set_err(PS_E_BAD_ARG, "store is NULL");
+    for (FcParams &p : s->ln)
+        if (layer < 0 && p.pending_cnt > 0) PSCHK(store_check_ln_update(s));
     PSCHK(store_enter(s));
     int done = 0;
     bool one = false;

@@ -105,6 +105,7 @@ static inline bool key_is_bias(const ParsedKey &k) { return k.kind == 4 || k.kin
 static inline bool key_is_ln(const ParsedKey &k) { return k.kind >= 5; }
 // KVStore.update of a dense tensor's pending gradient (ps_layer_ops.hip); false: it has none
 int store_apply_pending(ps_store *s, FcParams &p, const char *stem, int layer, bool *done);
+int store_check_ln_update(ps_store *s);          // refused while a graph is recorded
 #define PS_LN_MAX 64
 // the operators that know the reference's activations alone: the residual tower's would pass for none
 static inline int store_check_act(int act) {

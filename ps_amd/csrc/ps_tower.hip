@@ -186,6 +186,7 @@ extern "C" int ps_ln_update(ps_store_t *s, int layer) {
     if (!s) return ps_set_err(PS_E_BAD_ARG, "store is NULL");
     FcParams *p;
     PSCHK(find_ln(s, layer, &p));
+    if (p->pending_cnt > 0) PSCHK(store_check_ln_update(s));
     PSCHK(store_enter(s));
     bool done = false;
     PSCHK(store_apply_pending(s, *p, "ln", layer, &done));
