@@ -32,7 +32,7 @@ template <> struct Mma<float> {        // a fragment holds 4 steps of 2: the lan
 };
 
 // The normal law's tail Q(|z|) = erfc(|z| / sqrt 2) / 2 as 2 to a polynomial of |z|: log2 Q is nearly a parabola, and the polynomial is the
-// one of degree 10 whose error on [0, 8] is least, weighed as Q's own error or, where that is more, a twentieth of Q's in percent; it
+// one of degree 10 whose greatest error of Q on [0, 8], measured against the smaller of 2e-8 and Q / 1024, is least (0.3 of that); it
 // falls from there on.  In f32: |error| < 5e-8, the rounding of numbers near 1/2, and below 4e-4 of Q up to 8 (1e-6 up to 2, 6e-6 up to 3,
 // 4e-5 up to 4): a 16-bit GELU is its value rounded once down to -8, where it is 5e-15, and an ever smaller number below.  10
 // multiply-adds and one exponential: in the epilogue of a product nothing hides them.
